@@ -256,11 +256,11 @@ def _plain_beam(s):
   k, most, requests = min(n, V), s["most"], case["requests"]
   wide = x.double()
   top = wide.amax(1, keepdim=True)
-  norm = top + (wide - top).exp().sum(1, keepdim=True).log()
+  total = (wide - top).exp().sum(1, keepdim=True).log()
   del wide
   places = _rising(x) << 32 | (V - 1 - torch.arange(V, device=x.device))      # equal values: the lowest index first
   tokens = V - 1 - (places.topk(k, dim=1).values & 0xffffffff)
-  scores = s["cum"].double()[:, None] + (x.gather(1, tokens).double() - norm)
+  scores = s["cum"].double()[:, None] + (x.gather(1, tokens).double() - top - total)
   start = s["start"].long()
   rows = start[:-1, None] + torch.arange(most, device=x.device)
   there = rows < start[1:, None]
