@@ -1,0 +1,275 @@
+// Attention of a tree of new tokens over the paged cache, for any head size up to 640, any page size, float32 or bf16 storage, float32
+// arithmetic: the 32-bit path, and what the tensor-core kernel (attention_tree_tc.cu) does not take.  attention_tree.cuh says which keys a row
+// sees.
+//
+// A block has BR query rows of one (item, key/value head) and a piece of the item's keys, walked in tiles of BK: an online softmax in base 2,
+// scores and weighted values by FMAs from shared memory, 4 rows and BK / TX keys (then values) a thread, so a value read from shared
+// memory serves four products.  The rows of a head group lie side by side: a key is fetched once for all of them.  Pieces give a small
+// step enough blocks; more than one of them leave sums that tree_merge_kernel puts together.
+//
+// A key that a row does not see has the weight -1, which the weighted values leave out: a zero would make a NaN of an infinity there.
+//
+// What bounds it: FMAs, 4 a key, value and row, at half the rate, for every product needs its operands from shared memory.
+#include "attention_tree.cuh"
+
+namespace {
+
+using namespace mi_tree;
+
+constexpr int THREADS = 128;
+
+template <typename T>
+__device__ __forceinline__ void load_row4(float4& v, const T* p, int left, bool wide) {      // four values, zeros past the row
+  if (wide) {
+    if constexpr (sizeof(T) == 4) {
+      v = *reinterpret_cast<const float4*>(p);
+    } else {
+      const uint2 raw = *reinterpret_cast<const uint2*>(p);
+      v = make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u));
+    }
+  } else {
+    v = make_float4(mi::to_float(p[0]), left > 1 ? mi::to_float(p[1]) : 0.f, left > 2 ? mi::to_float(p[2]) : 0.f, left > 3 ? mi::to_float(p[3]) : 0.f);
+  }
+}
+
+// grid: (pieces, row tiles * nkv, items)
+template <typename T, int BR, int BK, int HD>
+__global__ void __launch_bounds__(THREADS)
+tree_kernel(Args a, int chunk, int pieces, int wide) {
+  constexpr int TX = THREADS / (BR / 4), KEYS = BK / TX, COLS = HD / (4 * TX);
+  static_assert(BK % TX == 0 && HD % (4 * TX) == 0 && TX <= 32, "a row's threads share a warp");
+  extern __shared__ __align__(16) float smem[];
+  const int hd4 = (a.hd + 3) / 4, stride = 4 * hd4 + 4;      // a row in shared memory, 16 bytes on for the banks
+  float *q_s = smem, *k_s = q_s + BR * stride, *p_s = k_s + BK * stride;      // [BR, stride], [BK, stride] (keys, then values), [BR, BK + 4]
+  constexpr int PS = BK + 4;
+  const int piece = blockIdx.x, head = blockIdx.y % a.nkv, r0 = blockIdx.y / a.nkv * BR;
+  mi::grid_dependency_sync();
+  const Item it = item_of(a, blockIdx.z);
+  const int rows = it.n * a.G;
+  if (r0 >= rows) return;
+  const int key_begin = piece * chunk, key_end = piece == pieces - 1 ? it.ctx : min(it.ctx, key_begin + chunk);
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const T* qkv = reinterpret_cast<const T*>(a.qkv);
+  const T* kv = reinterpret_cast<const T*>(a.kv);
+
+  for (int i = threadIdx.x; i < BR * hd4; i += THREADS) {
+    const int r = i / hd4, d = 4 * (i - r * hd4), row = r0 + r;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < rows) load_row4(v, qkv + (size_t)(it.row0 + row / a.G) * a.width + (size_t)(head * a.G + row % a.G) * a.hd + d, a.hd - d, wide);
+    *reinterpret_cast<float4*>(q_s + r * stride + d) = v;
+  }
+  // of this thread's four rows: the token's mask, and where its window begins
+  const int* mask[4];
+  int token[4], begin[4], pos[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    token[i] = min(r0 + 4 * ty + i, rows - 1) / a.G;
+    mask[i] = a.mask + (size_t)(it.row0 + token[i]) * a.words;
+    pos[i] = a.window > 0 ? a.positions[it.row0 + token[i]] : 0;
+    begin[i] = window_begin(a, pos[i]);
+  }
+  float m[4], l[4], acc[4][COLS][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
+  }
+  auto load_tile = [&](int key0, int which) {
+    for (int i = threadIdx.x; i < BK * hd4; i += THREADS) {
+      const int k = i / hd4, d = 4 * (i - k * hd4), key = key0 + k;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (key < key_end) {
+        const size_t row = (((size_t)page_of(a, it, key) * 2 + which) * a.nkv + head) * a.page_size + key % a.page_size;
+        load_row4(v, kv + row * a.hd + d, a.hd - d, wide);
+      }
+      *reinterpret_cast<float4*>(k_s + k * stride + d) = v;
+    }
+  };
+  for (int key0 = key_begin; key0 < key_end; key0 += BK) {
+    __syncthreads();
+    load_tile(key0, 0);
+    __syncthreads();
+    float s[4][KEYS];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j) s[i][j] = 0.f;
+#pragma unroll 2
+    for (int d = 0; d < 4 * hd4; d += 4) {
+      float4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(q_s + (4 * ty + i) * stride + d);
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j) {
+        const float4 k = *reinterpret_cast<const float4*>(k_s + (tx + TX * j) * stride + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i][j] = fmaf(q[i].w, k.w, fmaf(q[i].z, k.z, fmaf(q[i].y, k.y, fmaf(q[i].x, k.x, s[i][j]))));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float top = -INFINITY;
+      bool see[KEYS];
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j) {
+        const int key = key0 + tx + TX * j, node = key - it.start;
+        see[j] = key < key_end;
+        if (node < 0) {
+          see[j] = see[j] && key >= begin[i];
+        } else if (see[j]) {
+          see[j] = (mask[i][node >> 5] >> (node & 31)) & 1;
+          if (a.window > 0) see[j] = see[j] && a.positions[it.row0 + node] >= begin[i];
+        }
+        s[i][j] = logit2_exact(s[i][j], a.scale, a.softcap);
+        if (see[j]) top = fmaxf(top, s[i][j]);
+      }
+#pragma unroll
+      for (int o = TX / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float next = fmaxf(m[i], top), off = next == -INFINITY ? 0.f : next, alpha = exp2f(m[i] - off);
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j) {
+        const float p = exp2f(s[i][j] - off);
+        if (see[j]) part += p;
+        p_s[(4 * ty + i) * PS + tx + TX * j] = see[j] ? p : -1.f;
+      }
+      m[i] = next;
+      l[i] = l[i] * alpha + part;      // (this thread's keys; the row's threads are added up at the end)
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][c][e] *= alpha;
+    }
+    __syncthreads();
+    load_tile(key0, 1);
+    __syncthreads();
+    const bool all = key0 + BK <= min(it.start, key_end) && a.window <= 0;      // every row sees every key of the tile
+    const int near = min(BK, key_end - key0);
+    for (int k = 0; k < near; ++k) {
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = p_s[(4 * ty + i) * PS + k];
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) {
+        const int d = 4 * (tx + TX * c);
+        if (d >= 4 * hd4) break;
+        const float4 v = *reinterpret_cast<const float4*>(k_s + k * stride + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (all || !(p[i] < 0.f)) {
+            acc[i][c][0] = fmaf(p[i], v.x, acc[i][c][0]);
+            acc[i][c][1] = fmaf(p[i], v.y, acc[i][c][1]);
+            acc[i][c][2] = fmaf(p[i], v.z, acc[i][c][2]);
+            acc[i][c][3] = fmaf(p[i], v.w, acc[i][c][3]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int o = TX / 2; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+    const int row = r0 + 4 * ty + i;
+    if (row >= rows) continue;
+    const int h = head * a.G + row % a.G;
+    const size_t at = (size_t)(it.row0 + token[i]) * a.nh + h;
+    if (pieces > 1) {
+      const size_t slot = at * pieces + piece;
+      if (tx == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * (tx + TX * c) + e < a.hd) a.part_o[slot * a.hd + 4 * (tx + TX * c) + e] = acc[i][c][e];
+      continue;
+    }
+    const float sink2 = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
+    const float top = fmaxf(m[i], sink2), off = top == -INFINITY ? 0.f : top, weight = exp2f(m[i] - off);
+    const float total = l[i] * weight + exp2f(sink2 - off), factor = total == 0.f ? 0.f : weight / total;      // nothing visible: zeros
+#pragma unroll
+    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * (tx + TX * c) + e < a.hd) reinterpret_cast<T*>(a.out)[at * a.hd + 4 * (tx + TX * c) + e] = mi::from_float<T>(acc[i][c][e] * factor);
+  }
+}
+
+// The pieces of a row added up, a warp per (token, head): grid (T, ceil(nh / 4)).  Rows that belong to no item are left as they were.
+template <typename T>
+__global__ void __launch_bounds__(128)
+tree_merge_kernel(Args a, int chunk, int pieces) {
+  const int h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, t = blockIdx.x;
+  mi::grid_dependency_sync();
+  if (h >= a.nh) return;
+  int ctx = -1;
+  for (int b = lane; b < a.items; b += 32) {
+    const Item it = item_of(a, b);
+    if (t >= it.row0 && t < it.row0 + it.n) ctx = it.ctx;
+  }
+  ctx = __reduce_max_sync(0xffffffffu, ctx);
+  if (ctx < 0) return;
+  const int n = min((ctx + chunk - 1) / chunk, pieces);
+  const size_t at = (size_t)t * a.nh + h;
+  const float sink2 = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
+  float top = sink2;
+  for (int s = lane; s < n; s += 32) top = fmaxf(top, a.part_ml[2 * (at * pieces + s)]);
+  top = mi::warp_max(top);
+  const float off = top == -INFINITY ? 0.f : top;
+  float total = exp2f(sink2 - off);
+  for (int s = 0; s < n; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at * pieces + s));
+    total = fmaf(ml.y, exp2f(ml.x - off), total);
+  }
+  for (int d = lane; d < a.hd; d += 32) {
+    float sum = 0.f;
+    for (int s = 0; s < n; ++s) sum = fmaf(a.part_o[(at * pieces + s) * a.hd + d], exp2f(a.part_ml[2 * (at * pieces + s)] - off), sum);
+    reinterpret_cast<T*>(a.out)[at * a.hd + d] = mi::from_float<T>(total == 0.f ? 0.f : sum / total);
+  }
+}
+
+template <typename T, int BR, int BK, int HD>
+int launch(const Args& a, int chunk, int pieces, bool wide, cudaStream_t stream) {
+  const int stride = (a.hd + 3) / 4 * 4 + 4;
+  const size_t smem = ((size_t)(BR + BK) * stride + BR * (BK + 4)) * sizeof(float);
+  static bool ready[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return mi_fail("attention_tree: no current device");
+  if (!ready[dev]) {
+    const size_t most = ((size_t)(BR + BK) * (HD + 4) + BR * (BK + 4)) * sizeof(float);
+    if (cudaFuncSetAttribute(tree_kernel<T, BR, BK, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
+      return mi_fail("attention_tree: %zu bytes of shared memory were refused", most);
+    ready[dev] = true;
+  }
+  const int tiles = (a.max_q * a.G + BR - 1) / BR;
+  MI_REQUIRE((long long)tiles * a.nkv <= 65535, "attention_tree: %d rows of %d heads are too many for one launch", a.max_q * a.G, a.nkv);
+  if (mi::launch(tree_kernel<T, BR, BK, HD>, dim3(pieces, tiles * a.nkv, a.items), dim3(THREADS), smem, stream, a, chunk, pieces, (int)wide) != cudaSuccess)
+    return mi_fail("attention_tree: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  if (pieces > 1 && mi::launch(tree_merge_kernel<T>, dim3(a.T, (a.nh + 3) / 4), dim3(128), 0, stream, a, chunk, pieces) != cudaSuccess)
+    return mi_fail("attention_tree: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  MI_LAUNCH_OK("attention_tree");
+  return 0;
+}
+
+}  // namespace
+
+// Every item with up to max_q new tokens.  chunk: keys of a piece; pieces: of an item, whose last one takes all
+// keys that are left.
+// scratch: T * nh * pieces * (hd + 2) floats, 8-byte aligned; unused with one piece.
+MI_API int mi_attention_tree(void* out, const void* qkv, int dtype, const void* kv, const int* block_table, int bt_stride, const int* q_start,
+                             const int* q_len, const int* ctx_len, const int* seq_slot, const int* mask, int words, const int* positions,
+                             const float* sink, float* scratch, int items, int T, int width, int nh, int nkv, int hd, int pages, int page_size,
+                             int window, int max_q, float scale, float softcap, int chunk, int pieces, cudaStream_t stream) {
+  MI_REQUIRE(items >= 0 && items <= 65535 && T >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0 && hd > 0 && hd <= 640 && pages > 0 && page_size > 0 && bt_stride > 0,
+             "attention_tree: bad sizes items=%d T=%d heads=%d/%d hd=%d pages=%d of %d", items, T, nh, nkv, hd, pages, page_size);
+  MI_REQUIRE(max_q >= 0 && (long long)words * 32 >= max_q && chunk > 0 && pieces > 0 && pieces <= 65535 && (long long)max_q * (nh / nkv) <= 1 << 24, "attention_tree: bad sizes max_q=%d words=%d chunk=%d pieces=%d", max_q, words, chunk, pieces);
+  if (items == 0 || T == 0 || max_q == 0) return 0;
+  Args a{out, qkv, kv, block_table, bt_stride, q_start, q_len, ctx_len, seq_slot, mask, words, positions, sink,
+         scratch + (size_t)T * nh * pieces * 2, scratch, items, T, width, nh, nkv, nh / nkv, hd, pages, page_size, window, max_q, scale, softcap};
+  const int size = dtype == MI_F32 ? 4 : 2;
+  const bool wide = hd % 4 == 0 && (long long)width % 4 == 0 && (((uintptr_t)qkv | (uintptr_t)kv) % (4 * size)) == 0;
+  if (dtype == MI_F32) return hd <= 256 ? launch<float, 32, 64, 256>(a, chunk, pieces, wide, stream) : launch<float, 16, 32, 640>(a, chunk, pieces, wide, stream);
+  MI_REQUIRE(dtype == MI_BF16, "attention_tree: unknown type");
+  return hd <= 256 ? launch<__nv_bfloat16, 32, 64, 256>(a, chunk, pieces, wide, stream) : launch<__nv_bfloat16, 16, 32, 640>(a, chunk, pieces, wide, stream);
+}

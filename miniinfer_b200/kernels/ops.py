@@ -1325,6 +1325,132 @@ def sample(out: torch.Tensor, logits: torch.Tensor, temperature: torch.Tensor, t
                             _stream()), kernels=2)
 
 
+def _here(t: torch.Tensor, what: str) -> None:
+  """Refuses a tensor that is not on the current device, whose stream the launch goes to."""
+  if not t.is_cuda:
+    raise KernelError("the engine's kernels run on CUDA tensors only (got a CPU tensor)")
+  if t.device.index != torch.cuda.current_device():
+    raise KernelError(f"{what}: the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+  for t in others:
+    if t is not None and t.device != first.device:
+      raise KernelError(f"{what}: the tensors are on several devices ({first.device}, {t.device})")
+
+
+BEAM_MAX_BEST = 128     # the most places of a request that one selection fills
+
+
+def beam_select(tokens: torch.Tensor, parents: torch.Tensor, scores: torch.Tensor, logits: torch.Tensor, cum: torch.Tensor,
+                row_start: torch.Tensor, workspace=None) -> None:
+  """The n best continuations of every request over all of its beams and the vocabulary: ``score(r, v) = cum[r] +
+  log_softmax(logits[r])[v]`` over the rows ``row_start[i] .. row_start[i + 1] - 1`` of request i, the best first, of equal ones the
+  lower row, then the lower token.  ``tokens``, ``parents`` (rows of ``logits``) int32 and ``scores`` float32, all ``[requests, n]``;
+  ``logits [R, V]`` float32 or bfloat16, ``cum [R]`` float32, ``row_start [requests + 1]`` int32, rising.
+
+  A score that is minus infinity or no number is no candidate: a forbidden token, a beam with ``cum`` minus infinity, a row that holds
+  a NaN or plus infinity.  Places that are left get token -1, parent -1 and score minus infinity; so do requests without rows.  n is at
+  most ``BEAM_MAX_BEST``.  Sums and scores are made in 64 bits.  ``workspace`` (a ``Workspace``) lends the scratch; without it scratch is
+  allocated."""
+  if logits.dim() != 2 or tokens.dim() != 2 or row_start.dim() != 1 or row_start.shape[0] != tokens.shape[0] + 1:
+    raise KernelError("beam_select: logits must be [rows, vocabulary], the results [requests, n], row_start [requests + 1]")
+  (R, V), (requests, n) = logits.shape, tokens.shape
+  if parents.shape != tokens.shape or scores.shape != tokens.shape or cum.shape != (R,):
+    raise KernelError("beam_select: shapes do not match")
+  if not 1 <= n <= BEAM_MAX_BEST or V < 1:
+    raise KernelError(f"beam_select: n={n} places (1 .. {BEAM_MAX_BEST}) of {V} tokens")
+  dt = _dt(logits)
+  if requests == 0:
+    return
+  _same_device("beam_select", logits, tokens, parents, scores, cum, row_start)
+  _here(logits, "beam_select")
+  lib = common_lib()
+  lib.mi_beam_select_words.restype = ctypes.c_longlong
+  words = int(lib.mi_beam_select_words(R, V, n))
+  if workspace is not None:
+    scratch = workspace.buffer("beam_scratch", (max(words, 1),), torch.int64)
+    arrivals = workspace.zeros("beam_arrivals", requests, torch.int32)
+  else:
+    scratch = torch.empty(max(words, 1), dtype=torch.int64, device=logits.device)
+    arrivals = torch.zeros(requests, dtype=torch.int32, device=logits.device)
+  _check(lib, lib.mi_beam_select(_ptr(tokens, torch.int32), _ptr(parents, torch.int32), _ptr(scores, torch.float32), _ptr(logits), dt,
+                                 _ptr(cum, torch.float32), _ptr(row_start, torch.int32), _ptr(scratch), _ptr(arrivals), R, V, requests, n,
+                                 _stream()))
+
+
+MOVE_MAX_PAIRS = 4096   # the most pairs of one call of reorder_states or copy_cache_pages
+
+
+def _pairs(what: str, base: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *more: Optional[torch.Tensor]) -> int:
+  if src.dim() != 1 or src.shape != dst.shape:
+    raise KernelError(f"{what}: sources and destinations must be two lists of one length")
+  _same_device(what, base, src, dst, *more)
+  return src.shape[0]
+
+
+def reorder_states(state: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+  """``state[:, dst[k]] = state[:, src[k]]`` for a group's per-request states ``[layers, slots, ...]`` of any type, as if every source were
+  read before any destination is written: the beams of a request may change places.  ``src``, ``dst`` int32 ``[pairs]``, at most
+  ``MOVE_MAX_PAIRS``; a pair with an index out of range is left out (padding: -1), the destinations differ from one another."""
+  n = _pairs("reorder_states", state, src, dst)
+  if state.dim() < 2 or not state.is_contiguous():
+    raise KernelError("reorder_states: the states must be contiguous [layers, slots, ...]")
+  if n > MOVE_MAX_PAIRS:
+    raise KernelError(f"reorder_states: {n} pairs, at most {MOVE_MAX_PAIRS} go in one call")
+  if n == 0 or state.numel() == 0:
+    return
+  _here(state, "reorder_states")
+  lib = common_lib()
+  L, S = state.shape[:2]
+  none = ctypes.c_void_p(0)
+  _check(lib, lib.mi_move_places(_ptr(state), L, ctypes.c_longlong(S), ctypes.c_longlong(state.numel() // (L * S) * state.element_size()),
+                                 _ptr(src, torch.int32), _ptr(dst, torch.int32), none, 0, ctypes.c_longlong(0), n, _stream()))
+
+
+def copy_cache_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, filled: Optional[torch.Tensor] = None) -> None:
+  """Page ``dst[k]`` of every layer of a pool ``[layers, pages, 2, heads, page_size, head_dim]`` becomes a copy of page ``src[k]`` - whole, or
+  with ``filled [pairs]`` int32 its first ``filled[k]`` tokens.  As if every source were read before any destination is written, so pages may
+  also change places.  Indices int32, at most ``MOVE_MAX_PAIRS`` pairs; a pair with an index out of range is left out, the destinations
+  differ from one another."""
+  n = _pairs("copy_cache_pages", kv, src, dst, filled)
+  if kv.dim() != 6 or kv.shape[2] != 2 or not kv.is_contiguous():
+    raise KernelError(f"copy_cache_pages: the pool must be contiguous [layers, pages, 2, heads, page_size, head_dim], got {tuple(kv.shape)}")
+  if filled is not None and filled.shape != src.shape:
+    raise KernelError("copy_cache_pages: one filled length for each pair")
+  if n > MOVE_MAX_PAIRS:
+    raise KernelError(f"copy_cache_pages: {n} pairs, at most {MOVE_MAX_PAIRS} go in one call")
+  if n == 0 or kv.numel() == 0:
+    return
+  _here(kv, "copy_cache_pages")
+  lib = common_lib()
+  L, pages, _, heads, P, hd = kv.shape
+  row = hd * kv.element_size()
+  _check(lib, lib.mi_move_places(_ptr(kv), L, ctypes.c_longlong(pages), ctypes.c_longlong(2 * heads * P * row), _ptr(src, torch.int32),
+                                 _ptr(dst, torch.int32), _ptr(filled, torch.int32), P, ctypes.c_longlong(row), n, _stream()))
+
+
+def move_cache_rows(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, group_start: torch.Tensor, most: int) -> None:
+  """The keys and values of the tokens at ``dst[k]`` become those at ``src[k]``, in every layer of a pool ``[layers, pages, 2, heads, page_size,
+  head_dim]``; a place is ``page * page_size + offset``, as in a slot mapping.  What it is for: the accepted path of a drafted tree goes to the
+  front of the tree's rows.  ``group_start [groups + 1]`` int32, rising: the pairs of a group (a request) are moved as if all of its sources
+  were read before any of its destinations is written - ``most`` pairs at a time, in order, so ``most`` is at least a group's pairs, unless
+  no destination lies behind its source -, while different groups touch different places.  All indices int32; a pair with an
+  index out of range is left out, a group's destinations differ."""
+  n = _pairs("move_cache_rows", kv, src, dst, group_start)
+  if kv.dim() != 6 or kv.shape[2] != 2 or not kv.is_contiguous():
+    raise KernelError(f"move_cache_rows: the pool must be contiguous [layers, pages, 2, heads, page_size, head_dim], got {tuple(kv.shape)}")
+  if group_start.dim() != 1 or group_start.shape[0] < 1 or most < 1:
+    raise KernelError("move_cache_rows: group_start must be [groups + 1], most at least 1")
+  if n == 0 or kv.numel() == 0 or group_start.shape[0] == 1:
+    return
+  _here(kv, "move_cache_rows")
+  lib = common_lib()
+  L, pages, _, heads, P, hd = kv.shape
+  _check(lib, lib.mi_move_cache_rows(_ptr(kv), L, ctypes.c_longlong(pages), heads, P, ctypes.c_longlong(hd * kv.element_size()), _ptr(src, torch.int32),
+                                     _ptr(dst, torch.int32), _ptr(group_start, torch.int32), n, group_start.shape[0] - 1, int(most), _stream()))
+
+
 class AttentionBatch:
   """Device-side description of a step for the attention kernels (all int32).
 
@@ -1334,11 +1460,12 @@ class AttentionBatch:
   Lists the launchers need: ``prefill_tiles`` ((item, first row) of every ``PREFILL_TILE`` rows of the items
   with several new tokens), ``prefill_wide_tiles`` (the same in steps of ``PREFILL_WIDE_TILE``; optional: without it
   the tcgen05 prefill kernel never pairs blocks), ``decode_items`` (the items with exactly one new token), their
-  lengths and the largest context."""
+  lengths and the largest context.  For trees of new tokens (``tree_attention``): ``max_q_len``, the most new tokens of an
+  item, and ``tree_mask [tokens, words]``, bit j of a token's row saying that it sees the item's new token j."""
 
   __slots__ = ("token_item", "positions", "seq_slot", "q_start", "q_len", "ctx_len", "num_tokens", "num_items",
                "prefill_tiles", "num_prefill_tiles", "prefill_wide_tiles", "num_prefill_wide_tiles", "decode_items", "num_decode",
-               "max_ctx_len", "decode_chunk", "scratch")
+               "max_ctx_len", "decode_chunk", "scratch", "max_q_len", "tree_mask")
 
   def __init__(self, **kw):
     for k in self.__slots__:
@@ -1496,6 +1623,63 @@ def latent_attention(out: torch.Tensor, q: torch.Tensor, kv_layer: torch.Tensor,
     return
   rest = batch.without(prefill, decode)
   attention(out, q, kv_layer, block_table, rest, num_heads, 1, head_dim, scale, window, sink=sink, out_hd=out_hd)
+
+
+def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor, block_table: torch.Tensor, batch: AttentionBatch,
+                   num_heads: int, num_kv_heads: int, head_dim: int, scale: float, window: Optional[int] = None,
+                   sink: Optional[torch.Tensor] = None, softcap: float = 0.0) -> None:
+  """``attention`` for items whose new tokens are a tree of drafted ones: a token sees the item's context - the first ``ctx_len - q_len`` keys -
+  and those of the item's new tokens whose bit is set in its row of ``batch.tree_mask`` (its ancestors and itself), whose keys and values
+  lie behind the context in the item's pages, in the order of the rows, whatever their positions are.  ``window``: a token at position p
+  sees keys of positions above ``p - window`` only; a context key's position is its place, a new token's is ``batch.positions``.  ``sink``
+  and ``softcap`` as in ``attention``.  A row that sees nothing becomes zero; rows of no item stay as they were.
+
+  Of ``batch`` it reads ``q_start, q_len, ctx_len, seq_slot`` and ``tree_mask`` (int32; ``positions`` too with a window), ``num_items``,
+  ``max_q_len`` - no item has more new tokens -, ``max_ctx_len`` and ``scratch``."""
+  T, mask = qkv.shape[0], batch.tree_mask
+  if num_kv_heads < 1 or num_heads % num_kv_heads or not 0 < head_dim <= MAX_HEAD_DIM:
+    raise KernelError(f"tree_attention: {num_heads} heads over {num_kv_heads} of {head_dim}")
+  if out.shape != (T, num_heads * head_dim) or out.dtype != qkv.dtype or kv_layer.dtype != qkv.dtype or qkv.dim() != 2 or qkv.shape[1] < num_heads * head_dim:
+    raise KernelError("tree_attention: shapes or dtypes do not match")
+  if kv_layer.dim() != 5 or kv_layer.shape[1:] != (2, num_kv_heads, kv_layer.shape[3], head_dim):
+    raise KernelError(f"tree_attention: cache layer has shape {tuple(kv_layer.shape)}")
+  if block_table.dim() != 2 or mask is None or batch.max_q_len is None or batch.max_ctx_len is None:
+    raise KernelError("tree_attention: the batch needs a mask, its largest item and its longest context, the pages a block table")
+  if mask.dim() != 2 or mask.shape[0] != T or 32 * mask.shape[1] < batch.max_q_len:
+    raise KernelError(f"tree_attention: a mask of {tuple(mask.shape)} words for {T} rows of up to {batch.max_q_len} new tokens")
+  if sink is not None and (sink.shape != (num_heads,) or sink.dtype != torch.float32):
+    raise KernelError("tree_attention: the sinks must be one float32 per query head")
+  if softcap < 0:
+    raise KernelError(f"tree_attention: softcap={softcap} must not be negative")
+  if window is not None and window < 0:
+    raise KernelError(f"tree_attention: window={window} must not be negative")
+  if window and (batch.positions is None or batch.positions.shape != (T,)):
+    raise KernelError("tree_attention: a window needs the tokens' positions")
+  for t in (batch.q_start, batch.q_len, batch.ctx_len, batch.seq_slot):
+    if t.dim() != 1 or t.shape[0] < batch.num_items:
+      raise KernelError("tree_attention: the batch's lists are shorter than its items")
+  dt = _dt(qkv)
+  if T == 0 or batch.num_items == 0 or batch.max_q_len <= 0:
+    return
+  _same_device("tree_attention", qkv, out, kv_layer, block_table, mask, batch.q_start, batch.q_len, batch.ctx_len, batch.seq_slot, sink)
+  _here(qkv, "tree_attention")
+  lib = common_lib()
+  win, page_size = int(window or 0), kv_layer.shape[3]
+  # pieces of the keys: enough blocks for the GPU, none shorter than a tile
+  blocks = batch.num_items * num_kv_heads * -(-batch.max_q_len * (num_heads // num_kv_heads) // 32)
+  pieces = max(1, min(4 * _num_sms(qkv.device) // blocks, -(-batch.max_ctx_len // 64)))
+  chunk = -(-batch.max_ctx_len // pieces)
+  scratch = None
+  if pieces > 1:
+    n = T * num_heads * pieces * (head_dim + 2)
+    scratch = (batch.scratch.buffer("attention_tree_partials", (n,), torch.float32) if batch.scratch is not None
+               else torch.empty(n, dtype=torch.float32, device=qkv.device))
+  _check(lib, lib.mi_attention_tree(
+    _ptr(out), _ptr(qkv), dt, _ptr(kv_layer), _ptr(block_table, torch.int32), block_table.shape[1], _ptr(batch.q_start, torch.int32),
+    _ptr(batch.q_len, torch.int32), _ptr(batch.ctx_len, torch.int32), _ptr(batch.seq_slot, torch.int32), _ptr(mask, torch.int32), mask.shape[1],
+    _ptr(batch.positions if win else None, torch.int32), _ptr(sink), _ptr(scratch), batch.num_items, T, qkv.shape[1], num_heads, num_kv_heads, head_dim,
+    kv_layer.shape[0], page_size, win, int(batch.max_q_len), ctypes.c_float(scale), ctypes.c_float(softcap), chunk, pieces, _stream()),
+    kernels=1 + int(pieces > 1))
 
 
 class _AttentionOptions:

@@ -607,6 +607,84 @@ def sample(out, logits, temperature, top_k, top_p, seed, counter, workspace=None
       out[r] = int(torch.argmax(sc))
 
 
+def beam_select(tokens, parents, scores, logits, cum, row_start, workspace=None):
+  """In float64, one request after the other."""
+  n = tokens.shape[1]
+  every = torch.log_softmax(logits.double(), dim=1) + cum.double()[:, None]
+  every = torch.where(every.isnan(), torch.full_like(every, float("-inf")), every).cpu()
+  V = logits.shape[1]
+  for i, (lo, hi) in enumerate(zip(row_start.tolist(), row_start.tolist()[1:])):
+    flat = every[lo:hi].reshape(-1)
+    order = torch.argsort(flat, descending=True, stable=True)[:n]
+    order = order[flat[order] > float("-inf")]
+    tokens[i], parents[i], scores[i] = -1, -1, float("-inf")
+    k = order.numel()
+    tokens[i, :k] = (order % V).int().to(tokens.device)
+    parents[i, :k] = (lo + order // V).int().to(tokens.device)
+    scores[i, :k] = flat[order].float().to(tokens.device)
+
+
+def _in_range(src, dst, places):
+  return [(k, a, b) for k, (a, b) in enumerate(zip(src.tolist(), dst.tolist())) if 0 <= a < places and 0 <= b < places]
+
+
+def reorder_states(state, src, dst):
+  old = state.clone()
+  for _, a, b in _in_range(src, dst, state.shape[1]):
+    state[:, b] = old[:, a]
+
+
+def copy_cache_pages(kv, src, dst, filled=None):
+  old = kv.clone()
+  for k, a, b in _in_range(src, dst, kv.shape[1]):
+    n = kv.shape[4] if filled is None else max(0, int(filled[k]))
+    kv[:, b, :, :, :n] = old[:, a, :, :, :n]
+
+
+def move_cache_rows(kv, src, dst, group_start, most):
+  P, old = kv.shape[4], kv.clone()
+  first, last = int(group_start[0]), int(group_start[-1])
+  for k, a, b in _in_range(src, dst, kv.shape[1] * P):
+    if first <= k < last:
+      kv[:, b // P, :, :, b % P] = old[:, a // P, :, :, a % P]
+
+
+def tree_terms(qkv, kv_layer, block_table, batch, nh, nkv, hd, scale, window=None, sink=None, softcap=0.0):
+  """In float64, for every token: out [nh, hd]; sum of weight * |value|; the largest scale * sum |q| |k| of a key."""
+  P, G = kv_layer.shape[3], nh // nkv
+  q_start, q_len, ctx_len, slots = (x.tolist() for x in (batch.q_start, batch.q_len, batch.ctx_len, batch.seq_slot))
+  mask = batch.tree_mask.tolist()
+  got = {}
+  for b in range(batch.num_items):
+    r0, n, ctx = q_start[b], q_len[b], ctx_len[b]
+    start, keys = ctx - n, torch.arange(ctx)
+    pages = block_table[slots[b]].cpu().long()[keys // P].to(kv_layer.device)
+    k, v = (kv_layer[pages, w, :, (keys % P).to(kv_layer.device)].double().repeat_interleave(G, dim=1) for w in (0, 1))
+    where = keys.clone()
+    if window:
+      where[start:] = batch.positions[r0:r0 + n].cpu().long()
+    for i in range(n):
+      see = torch.tensor([1] * start + [mask[r0 + i][j // 32] >> j % 32 & 1 for j in range(n)], dtype=torch.bool)
+      if window:
+        see = see & (where > int(batch.positions[r0 + i]) - window)
+      at = see.nonzero()[:, 0].to(k.device)
+      q = qkv[r0 + i, :nh * hd].double().view(nh, hd)
+      z = torch.einsum("hd,nhd->hn", q, k[at]) * scale
+      size = (torch.einsum("hd,nhd->hn", q.abs(), k[at].abs()) * scale).amax(1) if at.numel() else torch.zeros(nh, dtype=torch.float64, device=q.device)
+      if softcap:
+        z = softcap * torch.tanh(z / softcap)
+      if sink is not None:
+        z = torch.cat((z, sink.double()[:, None]), dim=1)
+      w = torch.softmax(z, dim=1)[:, :at.numel()] if z.shape[1] else z
+      got[r0 + i] = (torch.einsum("hn,nhd->hd", w, v[at]), torch.einsum("hn,nhd->hd", w, v[at].abs()), size)
+  return got
+
+
+def tree_attention(out, qkv, kv_layer, block_table, batch, nh, nkv, hd, scale, window=None, sink=None, softcap=0.0):
+  for t, (o, _, _) in tree_terms(qkv, kv_layer, block_table, batch, nh, nkv, hd, scale, window, sink, softcap).items():
+    out[t] = o.reshape(-1).to(out.dtype)
+
+
 def install(monkeypatch) -> None:
   """Puts the statements above in place of the CUDA kernels (CPU tests of the host-side logic)."""
   from miniinfer_b200.kernels import ops
@@ -616,5 +694,5 @@ def install(monkeypatch) -> None:
                "add_rmsnorm_pair", "rms_pair_sum", "linear_batched", "causal_conv", "selective_scan", "gated_delta", "latent_down",
                "latent_query", "linear_attention", "hyper_connection", "relu_squared", "linear_relu_squared", "scaled_pair_sum",
                "glu_mul", "linear_glu", "linear_parts", "token_shift", "norm_scaled_add", "rglru_recurrence", "mingru_recurrence",
-               "residual_step", "softcap"):
+               "residual_step", "softcap", "beam_select", "reorder_states", "copy_cache_pages", "move_cache_rows", "tree_attention"):
     monkeypatch.setattr(ops, name, globals()[name])
