@@ -3,7 +3,7 @@
 // An item (a request) has `start` = ctx_len - q_len context keys and q_len new tokens, whose keys and values lie behind them in its pages:
 // token t's at place start + t, whatever its position is.  A token sees the context keys, those further than `window` positions back excepted,
 // and of the new ones those whose bit is set in its mask (a node's ancestors and itself).  A key's position is its place for the context and
-// positions[] for the new tokens.
+// positions[] for the new tokens - one of start .. ctx_len - 1.
 //
 // Query rows of one item and key/value head lie behind one another, [token, head of the group]: row = token * G + g.
 #pragma once

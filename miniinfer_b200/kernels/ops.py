@@ -1631,8 +1631,8 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
   """``attention`` for items whose new tokens are a tree of drafted ones: a token sees the item's context - the first ``ctx_len - q_len`` keys -
   and those of the item's new tokens whose bit is set in its row of ``batch.tree_mask`` (its ancestors and itself), whose keys and values
   lie behind the context in the item's pages, in the order of the rows, whatever their positions are.  ``window``: a token at position p
-  sees keys of positions above ``p - window`` only; a context key's position is its place, a new token's is ``batch.positions``.  ``sink``
-  and ``softcap`` as in ``attention``.  A row that sees nothing becomes zero; rows of no item stay as they were.
+  sees keys of positions above ``p - window`` only; a context key's position is its place, a new token's is ``batch.positions`` (its depth
+  on top of the context's length: one of the places that the item's new tokens have).  ``sink`` and ``softcap`` as in ``attention``.  A row that sees nothing becomes zero; rows of no item stay as they were.
 
   Of ``batch`` it reads ``q_start, q_len, ctx_len, seq_slot`` and ``tree_mask`` (int32; ``positions`` too with a window), ``num_items``,
   ``max_q_len`` - no item has more new tokens -, ``max_ctx_len`` and ``scratch``."""
@@ -1665,6 +1665,23 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
   _here(qkv, "tree_attention")
   lib = common_lib()
   win, page_size = int(window or 0), kv_layer.shape[3]
+  where = (_ptr(block_table, torch.int32), block_table.shape[1], _ptr(batch.q_start, torch.int32), _ptr(batch.q_len, torch.int32),
+           _ptr(batch.ctx_len, torch.int32), _ptr(batch.seq_slot, torch.int32), _ptr(mask, torch.int32), mask.shape[1],
+           _ptr(batch.positions if win else None, torch.int32), _ptr(sink))
+  sizes = (batch.num_items, T, qkv.shape[1], num_heads, num_kv_heads, head_dim, kv_layer.shape[0], page_size, win, int(batch.max_q_len),
+           ctypes.c_float(scale), ctypes.c_float(softcap))
+  if dt == BF16 and lib.mi_attention_tree_tc_takes(_ptr(out), _ptr(qkv), _ptr(kv_layer), T, qkv.shape[1], num_heads, num_kv_heads, head_dim,
+                                                   ctypes.c_longlong(kv_layer.shape[0]), page_size, int(batch.max_q_len), ctypes.c_float(scale)):
+    lib.mi_attention_tree_tc_floats.restype = ctypes.c_longlong
+    n = int(lib.mi_attention_tree_tc_floats(batch.num_items, num_heads, num_kv_heads, head_dim, int(batch.max_q_len)))
+    if batch.scratch is not None:
+      scratch, status = batch.scratch.buffer("attention_tree_partials", (n,), torch.float32), batch.scratch.zeros("attention_tree_status", 1, torch.int32)
+    else:
+      scratch, status = torch.empty(n, dtype=torch.float32, device=qkv.device), torch.zeros(1, dtype=torch.int32, device=qkv.device)
+    _check(lib, lib.mi_attention_tree_tc(_ptr(out), _ptr(qkv), _ptr(kv_layer), *where, _ptr(scratch), _ptr(status), *sizes, _stream()), kernels=2)
+    if batch.scratch is None and int(status[0]) != 0:
+      raise KernelError("tree_attention: a bounded wait on a barrier ran out")
+    return
   # pieces of the keys: enough blocks for the GPU, none shorter than a tile
   blocks = batch.num_items * num_kv_heads * -(-batch.max_q_len * (num_heads // num_kv_heads) // 32)
   pieces = max(1, min(4 * _num_sms(qkv.device) // blocks, -(-batch.max_ctx_len // 64)))
@@ -1674,12 +1691,8 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
     n = T * num_heads * pieces * (head_dim + 2)
     scratch = (batch.scratch.buffer("attention_tree_partials", (n,), torch.float32) if batch.scratch is not None
                else torch.empty(n, dtype=torch.float32, device=qkv.device))
-  _check(lib, lib.mi_attention_tree(
-    _ptr(out), _ptr(qkv), dt, _ptr(kv_layer), _ptr(block_table, torch.int32), block_table.shape[1], _ptr(batch.q_start, torch.int32),
-    _ptr(batch.q_len, torch.int32), _ptr(batch.ctx_len, torch.int32), _ptr(batch.seq_slot, torch.int32), _ptr(mask, torch.int32), mask.shape[1],
-    _ptr(batch.positions if win else None, torch.int32), _ptr(sink), _ptr(scratch), batch.num_items, T, qkv.shape[1], num_heads, num_kv_heads, head_dim,
-    kv_layer.shape[0], page_size, win, int(batch.max_q_len), ctypes.c_float(scale), ctypes.c_float(softcap), chunk, pieces, _stream()),
-    kernels=1 + int(pieces > 1))
+  _check(lib, lib.mi_attention_tree(_ptr(out), _ptr(qkv), dt, _ptr(kv_layer), *where, _ptr(scratch), *sizes, chunk, pieces, _stream()),
+         kernels=1 + int(pieces > 1))
 
 
 class _AttentionOptions:
@@ -1984,7 +1997,7 @@ def forget_tensors() -> None:
 def device_status(ws) -> int:
   """The status words that kernels with bounded waits set when a wait ran out (0: all well)."""
   code = 0
-  for name in ("attention_decode_counters", "attention_prefill_status", "gemm_tc_status", "chunked_state_status"):
+  for name in ("attention_decode_counters", "attention_prefill_status", "attention_tree_status", "gemm_tc_status", "chunked_state_status"):
     buf = ws._bufs.get((name, torch.int32))
     if buf is not None:
       code |= int(buf[0])
