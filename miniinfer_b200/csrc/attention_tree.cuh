@@ -35,7 +35,7 @@ struct Item {
 __device__ __forceinline__ Item item_of(const Args& a, int b) {
   Item it;
   it.row0 = max(a.q_start[b], 0);
-  it.ctx = max(a.ctx_len[b], 0);
+  it.ctx = (int)max(0ll, min((long long)a.ctx_len[b], (long long)a.bt_stride * a.page_size));
   it.n = min(min(a.q_len[b], a.max_q), min(it.ctx, a.T - it.row0));
   it.n = max(it.n, 0);
   it.start = it.ctx - it.n;

@@ -8,15 +8,16 @@
 // pieces of one that several share are left as sums that are not normalised, two at most a block, and tree_join_kernel adds them up.
 //
 // Roles of a block: a producer warp (queries of a unit, keys and values tile by tile into a ring of boxes, by TMA in the 128-byte swizzle;
-// a lane a box, the next tile's pages looked up ahead), a thread that issues all products, eight softmax warps.  Weights stay in tensor memory,
-// over the scores they come from.  With 128 rows (QT = 1) two score buffers take turns, scores run two tiles ahead, and two threads share a row;
-// with 256 (QT = 2, heads up to 128) two sets of rows take turns on one tile of keys, a thread a row, and keys and values are
-// fetched once for both.
+// a lane a box, the next tile's pages looked up ahead), a warp that issues all products, and two sets of four softmax warps, a thread a row, that take
+// turns on the tensor cores and on the exponentials: one set's scores are made while the other's weights are.  Weights stay in tensor memory, over the scores they come
+// from.  With up to 128 rows the sets are two streams of key tiles of the same rows, put together at the end of a piece; with up to 256 they are two sets of rows on
+// the same tiles, whose keys and values are fetched once for both.  Heads beyond 128 leave tensor memory for one set's sums only.
 //
 // Weights of invisible keys are zeros in P V, so whatever is not finite among the values of a tile that the mask touches is taken out in
 // shared memory first; a row that does see such a value gets it added at the end.  Only those tiles pay for it.
 //
-// The weight of the running maximum is exactly 1; weights are rounded to bf16, and the sum that divides the row is that of the rounded ones.
+// Weights are relative to a maximum that may lag behind the row's by 2^8, so that a row of sums is rescaled a few times and not in every tile; they are
+// rounded to bf16, and the sum that divides the row is that of the rounded ones.
 #include <cuda.h>
 #include <string.h>
 
@@ -27,16 +28,16 @@ namespace {
 using namespace mi_tree;
 
 constexpr int BM = 128, BOX = 64, BUFFERS = 2;
-constexpr int SOFTMAX_WARPS = 8, PRODUCER_WARP = 8, MMA_WARP = 9, THREADS = 320;
 constexpr int TMEM_COLS = 512, S_COL = 256;
 constexpr int MAX_UNITS = 12;                 // boxes of the ring: a tile's keys or its values each
 constexpr int WAIT_LIMIT = 1 << 22;
-constexpr int SMEM_BYTES = 227 << 10, SMEM_TAIL = 4096;      // behind queries and ring: barriers, maxima, sums
+constexpr int SMEM_BYTES = 227 << 10;
+constexpr int BARS = 76;                      // 8-byte words behind queries and ring: barriers, pieces
 
 struct Tc {
   Args a;
   int* status;
-  int2* units;                   // [items * nkv * max_parts]: first block, pieces
+  int4* joins;                   // [blocks]: of the unit that begins in a block and goes on in others: pieces, first token, tokens, key/value head
   int boxes, steps, n_out;       // boxes and 16s of columns of a row, columns of P V
   int ring, box_rows;            // units of the ring; rows of a TMA box of keys
   int tokens, max_parts;         // tokens of a set of 128 rows; parts of the largest item
@@ -79,6 +80,12 @@ __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int 
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// True in one thread of a warp that is together.
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
+  return yes != 0;
+}
 // The barrier gets an arrival when all products issued so far by this thread are done.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -115,6 +122,17 @@ __device__ __forceinline__ void tmem_ld(float (&v)[32], uint32_t taddr) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_ld(float (&v)[16], uint32_t taddr) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_ld(float (&v)[64], uint32_t taddr) {
   uint32_t r[64];
   asm volatile(
@@ -142,7 +160,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The line of tiles: item after item, in an item head after head, in a head part after part (QT * tokens tokens each).
+// The line of work: item after item, in an item head after head, in a head part after part (QT * tokens tokens each).  A unit takes its
+// tiles and `overhead` more in front of them: what queries, the first copies and the results cost, as long as a block has several tiles.
+constexpr int OVERHEAD = 4, OVERHEAD_FROM = 4;      // from that many tiles a block on
 struct Line {
   int t_begin, tiles, parts;     // of an item: first tile that some row sees, tiles, parts
 };
@@ -154,72 +174,97 @@ __device__ __forceinline__ Line line_of(const Tc& k, const Item& it) {
   l.parts = (it.n + QT * k.tokens - 1) / (QT * k.tokens);
   return l;
 }
-__device__ __forceinline__ long long stretch_begin(long long total, int b, int blocks) { return total * b / blocks; }
+// Block b's stretch: `base` places of the line, one more for the first `more` blocks; and the block that a place belongs to.
+__device__ __forceinline__ int stretch_begin(int base, int more, int b) { return b * base + min(b, more); }
+__device__ __forceinline__ int stretch_of(int base, int more, int place) {
+  const int longer = more * (base + 1);
+  return place < longer ? place / (base + 1) : more + (place - longer) / base;
+}
 
 // Where a block's stretch begins, and how long it is.
 struct Start {
-  int item, left;
-  long long offset, total;       // tiles of the item before the stretch; of the whole line
-  int blocks;                    // that have a stretch
+  Item it;                       // the first item
+  int item, left, offset;        // its number; places of the stretch; places of the item before it
 };
 
-// A stretch's next piece of a unit.
+// A piece of a unit: some of its tiles, as the producer describes it to the other warps.
 struct Piece {
   Item it;
-  Line l;
-  int b, head, part, j0, n;      // item, key/value head, part; first tile of the unit's, tiles
-  bool whole;
-  int slot;                      // of the sums, where the unit goes on in other blocks
+  int n, key;                    // tiles (0: no piece is left), first key
+  int head, first;               // key/value head; the unit's first token in the item
+  int slot;                      // of the sums, where the unit goes on in other blocks; -1: it does not
+  int pieces;                    // where it begins here and goes on: in how many blocks; else 0
 };
+constexpr int PIECES = 4;        // that are described at a time: the producer is at most two ahead of the last reader
+
 template <int QT, int BN>
 struct Walk {
   const Tc& k;
-  int item, left;
-  long long offset;
+  int item, left, offset, place, base, more, overhead;      // place: where on the line the walk is
   Item it;
   Line l;
-  bool first = true;
-  __device__ Walk(const Tc& k_, const Start& s) : k(k_), item(s.item), left(s.left), offset(s.offset) {
-    if (left > 0) load();
-  }
-  __device__ void load() {
-    it = item_of(k.a, item);
-    l = line_of<QT, BN>(k, it);
-  }
+  __device__ Walk(const Tc& k_, const Start& s, int place_, int base_, int more_, int overhead_)
+      : k(k_), item(s.item), left(s.left), offset(s.offset), place(place_), base(base_), more(more_), overhead(overhead_), it(s.it), l(line_of<QT, BN>(k_, s.it)) {}
   __device__ bool next(Piece& p) {
-    if (left <= 0) return false;
-    long long all = (long long)l.tiles * k.a.nkv * l.parts;
-    while (offset >= all) {      // (also items without tokens)
-      offset -= all;
-      if (++item >= k.a.items) return false;
-      load();
-      all = (long long)l.tiles * k.a.nkv * l.parts;
+    while (left > 0) {
+      const int all = (l.tiles + overhead) * k.a.nkv * l.parts;
+      if (offset >= all) {      // (also items without tokens)
+        offset -= all;
+        if (++item >= k.a.items) return false;
+        it = item_of(k.a, item);
+        l = line_of<QT, BN>(k, it);
+        continue;
+      }
+      const int unit = offset / (l.tiles + overhead), at = offset - unit * (l.tiles + overhead), n = min(left, (l.tiles + overhead) - at);      // places of the unit in this stretch
+      const int j0 = max(at - overhead, 0), j1 = max(at + n - overhead, 0), first_tile = place - at + overhead;
+      offset += n;
+      left -= n;
+      place += n;
+      if (j1 <= j0) continue;
+      p.it = it;
+      p.n = j1 - j0;
+      p.key = (l.t_begin + j0) * BN;
+      p.head = unit / l.parts;
+      const int part = unit - p.head * l.parts;
+      p.first = part * QT * k.tokens;
+      p.slot = p.n == l.tiles ? -1 : 2 * (int)blockIdx.x + (j0 == 0 ? 1 : 0);
+      p.pieces = p.n < l.tiles && j0 == 0 ? stretch_of(base, more, first_tile + l.tiles - 1) - (int)blockIdx.x + 1 : 0;
+      return true;
     }
-    const int unit = (int)(offset / l.tiles);
-    p.it = it;
-    p.l = l;
-    p.b = item;
-    p.head = unit / l.parts;
-    p.part = unit - p.head * l.parts;
-    p.j0 = (int)(offset - (long long)unit * l.tiles);
-    p.n = min(left, l.tiles - p.j0);
-    p.whole = p.n == l.tiles;
-    p.slot = 2 * (int)blockIdx.x + (p.j0 == 0 ? 1 : 0);
-    offset += p.n;
-    left -= p.n;
-    return true;
+    return false;
   }
 };
 
+// 2^x of two values on the multiply-add pipe: x = n + f with f in -1/2 .. 1/2 (adding 1.5 2^23 rounds to the whole number n), a cubic for 2^f
+// fitted to the smallest largest relative error, 1.0e-4, with value 1 at 0 - a twentieth of what rounding to bf16 does -, n added to the
+// exponent.  Below -127: exactly zero, as the cubic is 1 there.  The exponential unit takes 16 values a cycle and SM, and the 256 x 128 weights
+// of a tile 2048 cycles of it.
+__device__ __forceinline__ void ex2_cubic(float& x0, float& x1) {
+  float p0, p1, n0, n1;
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x0));      // -127; what is no number stays so
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x1));
+  asm("{\n .reg .b64 x, n, f, p, c;\n mov.b64 x, {%4, %5};\n mov.b64 c, {%6, %6};\n add.rn.f32x2 n, x, c;\n mov.b64 {%2, %3}, n;\n"
+      " mov.b64 c, {%7, %7};\n add.rn.f32x2 f, n, c;\n mov.b64 c, {%8, %8};\n fma.rn.f32x2 f, f, c, x;\n"
+      " mov.b64 p, {%9, %9};\n mov.b64 c, {%10, %10};\n fma.rn.f32x2 p, p, f, c;\n mov.b64 c, {%11, %11};\n fma.rn.f32x2 p, p, f, c;\n"
+      " mov.b64 c, {%12, %12};\n fma.rn.f32x2 p, p, f, c;\n mov.b64 {%0, %1}, p;\n}\n"
+      : "=f"(p0), "=f"(p1), "=f"(n0), "=f"(n1)
+      : "f"(x0), "f"(x1), "f"(12582912.f), "f"(-12582912.f), "f"(-1.f), "f"(0.055008747f), "f"(0.24221076f), "f"(0.69328290f), "f"(1.f));
+  x0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
+  x1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+}
+
 // Bits of the keys key0 .. key0 + 31 that a row sees: of the context from `begin` on, of the new ones by the token's mask (and the window).
-__device__ __forceinline__ uint32_t seen_bits(const Args& a, const Item& it, int key0, int begin, const int* mask) {
+// near: the mask's first 64 bits.
+__device__ __forceinline__ uint32_t seen_bits(const Args& a, const Item& it, int key0, int begin, const int* mask, uint64_t near) {
   auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
   uint32_t bits = below(it.start - key0) & ~below(begin - key0);
   const int j0 = key0 - it.start;
   if (j0 > -32 && j0 < it.n) {
     uint32_t nodes;
     if (j0 < 0) {
-      nodes = (uint32_t)mask[0] << -j0;
+      nodes = (uint32_t)near << -j0;
+    } else if (it.n <= 64) {
+      nodes = (uint32_t)(near >> j0);
     } else {
       const uint32_t lo = (uint32_t)mask[j0 >> 5], hi = (j0 >> 5) + 1 < a.words ? (uint32_t)mask[(j0 >> 5) + 1] : 0u;
       nodes = __funnelshift_r(lo, hi, j0 & 31);
@@ -237,10 +282,10 @@ __device__ __forceinline__ uint32_t seen_bits(const Args& a, const Item& it, int
 }
 
 // What the P V products have left out of a row's sums: values that are not finite, of keys that the row sees (a rare call).
-__device__ __noinline__ void add_not_finite(const Args& a, const Item& it, int head, int key_begin, int key_end, int begin, const int* mask, int col, float (&o)[32]) {
+__device__ __forceinline__ void add_not_finite(const Args& a, const Item& it, int head, int key_begin, int key_end, int begin, const int* mask, uint64_t near, int col, float (&o)[32]) {
   const __nv_bfloat16* kv = reinterpret_cast<const __nv_bfloat16*>(a.kv);
   for (int key0 = key_begin; key0 < key_end; key0 += 32) {
-    for (uint32_t bits = seen_bits(a, it, key0, begin, mask); bits; bits &= bits - 1) {
+    for (uint32_t bits = seen_bits(a, it, key0, begin, mask, near); bits; bits &= bits - 1) {
       const int key = key0 + __ffs(bits) - 1;
       if (key >= key_end) break;
       const __nv_bfloat16* v = kv + ((((size_t)page_of(a, it, key) * 2 + 1) * a.nkv + head) * a.page_size + key % a.page_size) * a.hd;
@@ -254,29 +299,38 @@ __device__ __noinline__ void add_not_finite(const Args& a, const Item& it, int h
   }
 }
 
-template <int QT, int BN>
-__global__ void __launch_bounds__(THREADS, 1)
+constexpr int threads_of(int sets) { return 32 * (4 * sets + 2); }
+
+template <int QT, int SETS, int BN, int STEPS>
+__global__ void __launch_bounds__(threads_of(SETS), 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const Tc k) {
-  constexpr int HALVES = 2 / QT, W = BN / HALVES;      // threads that share a row, their columns
+  constexpr int SOFTMAX_WARPS = 4 * SETS, PRODUCER_WARP = SOFTMAX_WARPS, MMA_WARP = SOFTMAX_WARPS + 1;
+  constexpr int N = 64;                                 // scores in registers at a time; their weights lie over the first half of them
+  constexpr int CUBIC = 1, CUBIC_OF = 4;                // pairs of weights of each four that are made without the exponential unit
   constexpr int COL_BYTES = BN * 128, Q_COL_BYTES = BM * 128;
-  constexpr int P_COUNT = SOFTMAX_WARPS / QT;
-  constexpr int LAG = QT == 1 ? 2 : 1;                  // tiles between two uses of a score buffer
-  constexpr int P_AT = QT == 1 ? 0 : 64;                // where in it the weights begin
   const Args& a = k.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* smem = smem_raw;             // aligned, for the kernel has no other shared memory; the ring leaves no room to move
+  if (smem_u32(smem) & 1023u) {
+    mi::grid_dependency_sync();
+    if (threadIdx.x == 0) {
+      atomicExch(k.status, 4);
+      k.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    return;
+  }
   const int q_bytes = k.boxes * Q_COL_BYTES, unit_bytes = k.boxes * COL_BYTES;      // of a set of rows; of a tile's keys or values
   unsigned char *q_s = smem, *ring_s = smem + QT * q_bytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring_s + k.ring * unit_bytes);
   uint64_t *q_full = bars, *q_empty = bars + 1, *o_free = bars + 2;
-  uint64_t *u_full = bars + 3, *u_empty = u_full + MAX_UNITS;
+  uint64_t *piece_full = bars + 3;                       // [PIECES]: described
+  uint64_t *u_full = piece_full + PIECES, *u_empty = u_full + MAX_UNITS;
   uint64_t *s_full = u_empty + MAX_UNITS, *p_full = s_full + BUFFERS, *o_full = p_full + BUFFERS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + BUFFERS);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* spoiled = abort + 1;      // [2]: the last piece, by parity, in which a value was not finite
-  Start* start = reinterpret_cast<Start*>(bars + 40);
-  float* row_max = reinterpret_cast<float*>(bars + 48);      // QT = 1: [2 tiles][2 halves][BM]; then the halves' sums [2][BM]
-  float* row_sum = row_max + 4 * BM;
+  Piece* pieces = reinterpret_cast<Piece*>(bars + 44);
+  float2* of_set = reinterpret_cast<float2*>(bars + BARS);      // [2][BM]: a row's maximum and sum in each stream of keys, at a piece's end
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -286,9 +340,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       mbar_init(&u_full[u], 1);
       mbar_init(&u_empty[u], 1);
     }
+    for (int i = 0; i < PIECES; ++i) mbar_init(&piece_full[i], 1);
     for (int b = 0; b < BUFFERS; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&p_full[b], P_COUNT);
+      mbar_init(&p_full[b], 4);      // the warps of a set
       mbar_init(&o_full[b], 1);
     }
     *abort = 0;
@@ -300,314 +355,352 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   mi::grid_dependency_sync();
-  if (warp == PRODUCER_WARP) {      // where this block's stretch of the line begins
-    auto tiles_of = [&](int b) {
-      if (b >= a.items) return 0ll;
-      const Line l = line_of<QT, BN>(k, item_of(a, b));
-      return (long long)l.tiles * a.nkv * l.parts;
-    };
-    auto scan = [&](long long x) {      // sums up to and with this lane
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      return x;
-    };
-    const long long mine0 = tiles_of(lane);      // the first 32 items stay in registers
-    long long total = __shfl_sync(0xffffffffu, scan(mine0), 31);
-    for (int b0 = 32; b0 < a.items; b0 += 32) total += __shfl_sync(0xffffffffu, scan(tiles_of(b0 + lane)), 31);
-    const int blocks = (int)min(total, (long long)gridDim.x), me = (int)blockIdx.x;
-    const long long begin = me < blocks ? stretch_begin(total, me, blocks) : total, end = me < blocks ? stretch_begin(total, me + 1, blocks) : total;
-    long long before = 0;
-    Start s{0, (int)(end - begin), 0, total, blocks};
-    for (int b0 = 0; b0 < a.items; b0 += 32) {
-      const long long mine = b0 ? tiles_of(b0 + lane) : mine0, upto = before + scan(mine);
-      const unsigned m = __ballot_sync(0xffffffffu, upto > begin);
-      if (m) {
-        const int at = __ffs(m) - 1;
-        s.item = b0 + at;
-        s.offset = begin - __shfl_sync(0xffffffffu, upto - mine, at);
-        break;
-      }
-      before = __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (lane == 0) *start = s;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walk<QT, BN> walk(k, *start);
-  Piece p;
-  // The ring's units of a piece of n tiles, counted from its first: in the order in which they are used.
-  auto key_unit = [](int j) { return QT == 1 ? (j == 0 ? 0 : 2 * j - 1) : 2 * j; };
-  auto value_unit = [](int j, int n) { return QT == 1 ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; };
+  // The values of tile j of a piece of n tiles, as a unit of the ring counted from the piece's first.
+  constexpr bool KEYS = QT == 1 && SETS == 2;           // the sets are streams of keys
+  auto value_unit = [](int j, int n) { return KEYS ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; };
 
   if (warp == PRODUCER_WARP) {
+    // where this block's stretch of the line begins
+    int overhead = 0;
+    auto places_of = [&](const Item& it) {
+      const Line l = line_of<QT, BN>(k, it);
+      return it.n > 0 ? (l.tiles + overhead) * a.nkv * l.parts : 0;
+    };
+    auto item_at = [&](int b) { return b < a.items ? item_of(a, b) : Item{0, 0, 0, 0, nullptr}; };
+    auto scan = [&](int x) {      // sums up to and with this lane
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      return x;
+    };
+    const Item mine0 = item_at(lane);      // the first 32 items stay in registers
+    auto all_places = [&]() {
+      int x = places_of(mine0);
+      for (int b0 = 32; b0 < a.items; b0 += 32) x += places_of(item_at(b0 + lane));
+      return __reduce_add_sync(0xffffffffu, x);
+    };
+    int total = all_places();
+    if (total >= OVERHEAD_FROM * (int)gridDim.x) {
+      overhead = OVERHEAD;
+      total = all_places();
+    }
+    const int upto0 = scan(places_of(mine0));
+    const int me = (int)blockIdx.x, base = total / (int)gridDim.x, more = total - base * (int)gridDim.x;
+    const int begin = stretch_begin(base, more, me);
+    Start from{Item{0, 0, 0, 0, nullptr}, 0, 0, 0};
+    int before = 0;
+    for (int b0 = 0; b0 < a.items; b0 += 32) {
+      const Item mine = b0 ? item_at(b0 + lane) : mine0;
+      const int upto = b0 ? before + scan(places_of(mine)) : upto0;
+      const unsigned m = __ballot_sync(0xffffffffu, upto > begin);
+      if (m) {
+        const int at = __ffs(m) - 1, prior = __shfl_sync(0xffffffffu, upto, max(at - 1, 0));
+        from.it = Item{__shfl_sync(0xffffffffu, mine.row0, at), __shfl_sync(0xffffffffu, mine.n, at), __shfl_sync(0xffffffffu, mine.start, at),
+                       __shfl_sync(0xffffffffu, mine.ctx, at), reinterpret_cast<const int*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine.bt), at))};
+        from.item = b0 + at;
+        from.left = base + (me < more ? 1 : 0);
+        from.offset = begin - (at > 0 ? prior : before);
+        break;
+      }
+      before = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    Walk<QT, BN> walk(k, from, begin, base, more, overhead);
     const int per_tile = BN / k.box_rows, loads = per_tile * k.boxes;      // a lane's box: rows and columns of the tile (16 boxes at most)
     const int rows = k.tokens * a.G;
-    long long u0 = 0;
-    int it = 0;
+    int4 joined = make_int4(0, 0, 0, 0);      // for the kernel that joins pieces
+    int slot = 0, turn = 1, it = 0;      // the ring's next unit; the parity that its barrier of free units is waited with
     auto stopped = [&]() { return __shfl_sync(0xffffffffu, *abort, 0) != 0; };      // the same answer for all lanes, which go on together
-    while (walk.next(p) && !stopped()) {
+    for (;; ++it) {
+      Piece p;
+      const bool more_pieces = walk.next(p);
+      if (!more_pieces) p.n = 0;
       const int* bt = p.it.bt;
       const int row = lane / k.boxes * k.box_rows, column = lane % k.boxes;
       auto page_at = [&](int j) {
-        const int key = (p.l.t_begin + p.j0 + j) * BN + row;
+        const int key = p.key + j * BN + row;
         return lane < loads && j < p.n ? min(max(bt[min(key / a.page_size, a.bt_stride - 1)], 0), a.pages - 1) : 0;
       };
-      int page = page_at(0), before = 0;
+      int page = page_at(0), behind = 0;
       mbar_wait(q_empty, (it & 1) ^ 1, abort, k.status);
+      if (stopped()) break;
       if (lane == 0) {
+        pieces[it % PIECES] = p;
+        mbar_arrive(&piece_full[it % PIECES]);
+      }
+      if (!more_pieces) break;
+      if (lane == 0) {
+        if (p.pieces) joined = make_int4(p.pieces, p.it.row0 + p.first, min(p.it.n - p.first, QT * k.tokens), p.head);
         mbar_expect_tx(q_full, (uint32_t)(QT * k.boxes * rows * 128));
         for (int s = 0; s < QT; ++s)
           for (int c = 0; c < k.boxes; ++c)
-            tma_load(q_s + s * q_bytes + c * Q_COL_BYTES, &q_map, c * BOX, p.head * a.G, p.it.row0 + (p.part * QT + s) * k.tokens, q_full);
+            tma_load(q_s + s * q_bytes + c * Q_COL_BYTES, &q_map, c * BOX, p.head * a.G, p.it.row0 + p.first + s * k.tokens, q_full);
       }
-      auto load = [&](int unit, int j, int page_id, int which) {
-        const long long u = u0 + unit;
-        const int s = (int)(u % k.ring);
-        mbar_wait(&u_empty[s], (uint32_t)((u / k.ring) & 1) ^ 1, abort, k.status);
+      auto load = [&](int j, int page_id, int which) {
+        const int s = slot;
+        mbar_wait(&u_empty[s], (uint32_t)turn, abort, k.status);
+        if (++slot == k.ring) {
+          slot = 0;
+          turn ^= 1;
+        }
         if (lane == 0) mbar_expect_tx(&u_full[s], (uint32_t)unit_bytes);
         __syncwarp();
         if (lane < loads && !*abort) {
-          const int key = (p.l.t_begin + p.j0 + j) * BN + row;
+          const int key = p.key + j * BN + row;
           const int y = ((page_id * 2 + which) * a.nkv + p.head) * a.page_size + key % a.page_size;      // (fits: the launcher asks for it)
           tma_load(ring_s + s * unit_bytes + column * COL_BYTES + row * 128, &kv_map, column * BOX, y, &u_full[s]);
         }
       };
       for (int j = 0; j < p.n && !stopped(); ++j) {
         const int next = page_at(j + 1);
-        load(key_unit(j), j, page, 0);
-        if constexpr (QT == 1) {
-          if (j > 0) load(value_unit(j - 1, p.n), j - 1, before, 1);
-          if (j == p.n - 1) load(value_unit(j, p.n), j, page, 1);
+        load(j, page, 0);
+        if constexpr (KEYS) {      // in the order in which they are used: keys run a tile ahead
+          if (j > 0) load(j - 1, behind, 1);
+          if (j == p.n - 1) load(j, page, 1);
         } else {
-          load(value_unit(j, p.n), j, page, 1);
+          load(j, page, 1);
         }
-        before = page;
+        behind = page;
         page = next;
       }
-      u0 += 2 * p.n;
-      ++it;
     }
+    if (lane == 0) k.joins[me] = joined;
   } else if (warp == MMA_WARP) {
-    if (lane == 0) {
+    {      // the whole warp goes through the waits together, one elected thread issues: descriptors then stay in uniform registers
+      auto stopped = [&]() { return __shfl_sync(0xffffffffu, *abort, 0) != 0; };
       constexpr uint32_t IDESC_S = instr_desc(BM, BN, false);
       const uint32_t idesc_pv = instr_desc(BM, k.n_out, true);
-      long long u0 = 0;
-      int g0 = 0, it = 0;
-      auto wait_unit = [&](int unit) {
-        const long long u = u0 + unit;
-        mbar_wait(&u_full[(int)(u % k.ring)], (uint32_t)((u / k.ring) & 1), abort, k.status);
-        return smem_u32(ring_s + (int)(u % k.ring) * unit_bytes);
+      int done[2] = {0, 0}, it = 0, slot = 0, turn = 0;      // tiles of a set
+      auto next_unit = [&]() {      // the ring's next unit, once it is there
+        const int s = slot;
+        mbar_wait(&u_full[s], (uint32_t)turn, abort, k.status);
+        if (++slot == k.ring) {
+          slot = 0;
+          turn ^= 1;
+        }
+        return s;
       };
-      auto free_unit = [&](int unit) { tc_commit(&u_empty[(int)((u0 + unit) % k.ring)]); };
+      auto unit_at = [&](int s) { return smem_u32(ring_s + s * unit_bytes); };
+      auto free_unit = [&](int s) {
+        if (elected()) tc_commit(&u_empty[s]);
+        __syncwarp();
+      };
       auto scores = [&](int set, int buffer, uint32_t keys) {
         const uint64_t q_desc = smem_desc(smem_u32(q_s + set * q_bytes), 16, 1024), k_desc = smem_desc(keys, 16, 1024);
-        for (int s = 0; s < k.steps; ++s) {
-          const int in_box = (s & 3) * 2;      // 16 columns further: 32 bytes of a row of its box
-          tc_mma(tmem + S_COL + BN * buffer, q_desc + (uint64_t)((s >> 2) * (Q_COL_BYTES >> 4) + in_box),
-                 k_desc + (uint64_t)((s >> 2) * (COL_BYTES >> 4) + in_box), IDESC_S, s > 0 ? 1u : 0u);
+        if (elected()) {
+          auto step = [&](int s) {      // 16 columns further: 32 bytes of a row of its box
+            const int in_box = (s & 3) * 2;
+            tc_mma(tmem + S_COL + BN * buffer, q_desc + (uint64_t)((s >> 2) * (Q_COL_BYTES >> 4) + in_box),
+                   k_desc + (uint64_t)((s >> 2) * (COL_BYTES >> 4) + in_box), IDESC_S, s > 0 ? 1u : 0u);
+          };
+          if constexpr (STEPS > 0) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) step(s);
+          } else {
+            for (int s = 0; s < k.steps; ++s) step(s);
+          }
+          tc_commit(&s_full[buffer]);
         }
-        tc_commit(&s_full[buffer]);
+        __syncwarp();
       };
       auto add = [&](int set, int buffer, uint32_t values, bool onto) {
         const uint64_t v_desc = smem_desc(values, COL_BYTES, 1024);
-        for (int s = 0; s < BN / 16; ++s)      // 16 keys further: 2048 bytes of every box
-          tc_mma_ts(tmem + 128 * set, tmem + S_COL + BN * buffer + P_AT + 8 * s, v_desc + (uint64_t)(s * (2048 >> 4)), idesc_pv, (onto || s > 0) ? 1u : 0u);
-        tc_commit(&o_full[buffer]);
+        if (elected()) {
+#pragma unroll
+          for (int s = 0; s < BN / 16; ++s)      // 16 keys further: 2048 bytes of every box
+            tc_mma_ts(tmem + 128 * set, tmem + S_COL + BN * buffer + 16 * s / 64 * 64 + 16 * s % 64 / 2, v_desc + (uint64_t)(s * (2048 >> 4)), idesc_pv, (onto || s > 0) ? 1u : 0u);
+          tc_commit(&o_full[buffer]);
+        }
+        __syncwarp();
       };
-      while (walk.next(p) && !*abort) {
-        const int n = p.n;
+      auto commit = [&](uint64_t* bar) {
+        if (elected()) tc_commit(bar);
+        __syncwarp();
+      };
+      for (;; ++it) {
+        mbar_wait(&piece_full[it % PIECES], (it / PIECES) & 1, abort, k.status);
+        const int n = stopped() ? 0 : pieces[it % PIECES].n;
+        if (n == 0) break;
         mbar_wait(q_full, it & 1, abort, k.status);
         tc_fence_after();
         if constexpr (QT == 1) {
           auto ahead = [&](int j) {
-            const uint32_t keys = wait_unit(key_unit(j));
-            if (*abort) return;
+            const int keys = next_unit();
+            if (stopped()) return;
             tc_fence_after();
-            scores(0, (g0 + j) & 1, keys);
-            free_unit(key_unit(j));
-            if (j == n - 1) tc_commit(q_empty);
+            scores(0, j % SETS, unit_at(keys));
+            free_unit(keys);
+            if (j == n - 1) commit(q_empty);
           };
-          for (int j = 0; j < min(n, 2) && !*abort; ++j) ahead(j);
-          for (int j = 0; j < n && !*abort; ++j) {
-            const int g = g0 + j;
+          for (int j = 0; j < min(n, SETS) && !stopped(); ++j) ahead(j);
+          for (int j = 0; j < n && !stopped(); ++j) {
+            const int set = j % SETS;
             if (j == 0 && it > 0) mbar_wait(o_free, (it - 1) & 1, abort, k.status);      // the piece before has its sums in registers
-            const uint32_t values = wait_unit(value_unit(j, n));
-            mbar_wait(&p_full[g & 1], (g >> 1) & 1, abort, k.status);
-            if (*abort) break;
+            const int values = next_unit();
+            mbar_wait(&p_full[set], done[set] & 1, abort, k.status);
+            ++done[set];
+            if (stopped()) break;
             tc_fence_after();
-            add(0, g & 1, values, j > 0);
-            free_unit(value_unit(j, n));
-            if (j + 2 < n) ahead(j + 2);
+            add(set, set, unit_at(values), j >= SETS);
+            free_unit(values);
+            if (j + SETS < n) ahead(j + SETS);
           }
         } else {
-          uint32_t keys = wait_unit(key_unit(0));
-          if (*abort) break;
+          int keys = next_unit();
+          if (stopped()) break;
           tc_fence_after();
-          scores(0, 0, keys);
-          scores(1, 1, keys);
-          free_unit(key_unit(0));
-          if (n == 1) tc_commit(q_empty);
-          for (int j = 0; j < n && !*abort; ++j) {
-            const int g = g0 + j;
+          scores(0, 0, unit_at(keys));
+          scores(1, 1, unit_at(keys));
+          free_unit(keys);
+          if (n == 1) commit(q_empty);
+          for (int j = 0; j < n && !stopped(); ++j) {
+            const int g = done[0] + j;
             if (j == 0 && it > 0) mbar_wait(o_free, (it - 1) & 1, abort, k.status);
-            const uint32_t values = wait_unit(value_unit(j, n));
+            const int values = next_unit();
             mbar_wait(&p_full[0], g & 1, abort, k.status);
-            if (*abort) break;
+            if (stopped()) break;
             tc_fence_after();
-            add(0, 0, values, j > 0);
+            add(0, 0, unit_at(values), j > 0);
             if (j + 1 < n) {
-              keys = wait_unit(key_unit(j + 1));
-              if (*abort) break;
+              keys = next_unit();
+              if (stopped()) break;
               tc_fence_after();
-              scores(0, 0, keys);
+              scores(0, 0, unit_at(keys));
             }
             mbar_wait(&p_full[1], g & 1, abort, k.status);
-            if (*abort) break;
+            if (stopped()) break;
             tc_fence_after();
-            add(1, 1, values, j > 0);
-            free_unit(value_unit(j, n));
+            add(1, 1, unit_at(values), j > 0);
+            free_unit(values);
             if (j + 1 < n) {
-              scores(1, 1, keys);
-              free_unit(key_unit(j + 1));
-              if (j + 2 == n) tc_commit(q_empty);
+              scores(1, 1, unit_at(keys));
+              free_unit(keys);
+              if (j + 2 == n) commit(q_empty);
             }
           }
         }
-        u0 += 2 * n;
-        g0 += n;
-        ++it;
+        if constexpr (QT == 2) done[0] += n;
       }
     }
-  } else {
-    // Warp w: tensor-memory lanes 32 (w % 4) .. + 31.  QT = 1: columns W (w / 4) .. of their rows; QT = 2: all columns of set w / 4's rows.
-    const int quarter = warp & 3, upper = warp >> 2, half = QT == 1 ? upper : 0, set = QT == 1 ? 0 : upper, r = quarter * 32 + lane;
-    const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t o_addr = t_lane + 128 * set;
-    int done[BUFFERS] = {};
-    auto wait_o = [&](int g) {      // P V of tile g is added
-      const int b = QT == 1 ? g & 1 : set, use = QT == 1 ? g >> 1 : g;
-#pragma unroll
-      for (int x = 0; x < BUFFERS; ++x)
-        if (x == b) {
-          while (done[x] <= use) {
-            mbar_wait(&o_full[x], done[x] & 1, abort, k.status);
-            ++done[x];
-          }
-        }
-      tc_fence_after();
-    };
-    auto meet = [&]() {      // the two warps that share rows
-      if constexpr (QT == 1) asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+  } else if (warp < SOFTMAX_WARPS) {
+    // Warp w: set w / 4, tensor-memory lanes 32 (w % 4) .. + 31, a thread a row.
+    const int quarter = warp & 3, set = warp >> 2, rows_set = QT == 2 ? set : 0, r = quarter * 32 + lane;
+    const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16), o_addr = t_lane + 128 * set, s_addr = t_lane + S_COL + BN * set;
+    auto sync_softmax = [&]() { asm volatile("bar.sync 9, %0;" ::"n"(32 * SOFTMAX_WARPS) : "memory"); };
+    auto any_of_softmax = [&](bool x) {
+      int any;
+      asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 9, %2, p;\n selp.b32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"((int)x), "n"(32 * SOFTMAX_WARPS) : "memory");
+      return any != 0;
     };
     const float factor = a.softcap > 0.f ? 1.f : k.scale_log2;      // capped scores come in base 2
-    long long u0 = 0;
-    int g = 0, it = 0;
-    while (walk.next(p)) {
-      const int tokens_left = p.it.n - (p.part * QT + set) * k.tokens, rows = min(max(tokens_left, 0), k.tokens) * a.G;
+    int g = 0, it = 0, u0 = 0;      // g: tiles of the set
+    for (;; ++it) {
+      mbar_wait(&piece_full[it % PIECES], (it / PIECES) & 1, abort, k.status);
+      if (any_of_softmax(*abort)) break;      // together: they meet at barriers below
+      const Piece& p = pieces[it % PIECES];
+      const int tiles = p.n;
+      if (tiles == 0) break;
+      const int rows = min(max(p.it.n - (p.first + rows_set * k.tokens), 0), k.tokens) * a.G;
       const bool valid = r < rows, busy = quarter * 32 < rows;      // this row exists; one of the warp's does
-      const int token = min(p.it.row0 + (p.part * QT + set) * k.tokens + r / a.G, p.it.row0 + p.it.n - 1);
+      const int token = min(p.it.row0 + p.first + rows_set * k.tokens + r / a.G, p.it.row0 + p.it.n - 1);
       const int* mask = a.mask + (size_t)token * a.words;
+      const uint64_t near = (uint32_t)mask[0] | (a.words > 1 ? (uint64_t)(uint32_t)mask[1] << 32 : 0ull);
       const int begin = a.window > 0 ? window_begin(a, a.positions[token]) : 0;
       // keys that the mask may hide from some row: the new ones and what lies behind, with a window those that it has passed for the last token
       const int hidden_from = p.it.start, hidden_to = a.window > 0 ? p.it.start + p.it.n - a.window : 0;
       float m_run = -INFINITY, l_run = 0.f;
-      int touched = 0x7fffffff;      // first key of the first tile that the mask touched
-      for (int j = 0; j < p.n; ++j, ++g) {
-        const int b = QT == 1 ? g & 1 : set, key0 = (p.l.t_begin + p.j0 + j) * BN;
+      for (int j = KEYS ? set : 0; j < tiles; j += KEYS ? 2 : 1, ++g) {
+        const bool first_of_set = j < SETS;
+        const int key0 = p.key + j * BN;
         const bool masked = key0 + BN > hidden_from || key0 < hidden_to;
-        const uint32_t s_addr = t_lane + S_COL + BN * b;
-        mbar_wait(&s_full[b], QT == 1 ? (g >> 1) & 1 : g & 1, abort, k.status);
+        uint32_t bits[BN / 32];      // keys that the row sees
+        if (masked && busy) {
+#pragma unroll
+          for (int i = 0; i < BN / 32; ++i) bits[i] = seen_bits(a, p.it, key0 + 32 * i, begin, mask, near);
+        }
+        mbar_wait(&s_full[set], g & 1, abort, k.status);
         tc_fence_after();
         if (masked) {      // values that are not finite are taken out before P V multiplies them with weights of zero
           // (behind the scores: the ring's earlier uses of this unit are over then, so the barrier's parity is this one's)
-          if (touched > key0) touched = key0;
-          const long long u = u0 + value_unit(j, p.n);
-          mbar_wait(&u_full[(int)(u % k.ring)], (uint32_t)((u / k.ring) & 1), abort, k.status);
-          unsigned char* v_s = ring_s + (int)(u % k.ring) * unit_bytes;
-          bool any = false;
-          for (int i = threadIdx.x; i < unit_bytes / 16; i += 32 * SOFTMAX_WARPS) {
-            uint4 x = *reinterpret_cast<const uint4*>(v_s + 16 * i);
-            uint32_t* w4 = &x.x;
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t hit = __vcmpeq2(w4[e] & 0x7f807f80u, 0x7f807f80u);
-              bad |= hit != 0;
-              w4[e] &= ~hit;
-            }
-            if (bad) {
-              *reinterpret_cast<uint4*>(v_s + 16 * i) = x;
-              any = true;
-            }
+          const int u = u0 + value_unit(j, tiles), turn = u / k.ring, unit = u - turn * k.ring;
+          mbar_wait(&u_full[unit], (uint32_t)(turn & 1), abort, k.status);
+          unsigned char* v_s = ring_s + unit * unit_bytes;
+          constexpr int STEP = KEYS ? BM : 32 * SOFTMAX_WARPS;
+          const int at0 = KEYS ? r : threadIdx.x;
+          const __nv_bfloat162 nought = __floats2bfloat162_rn(0.f, 0.f);
+          __nv_bfloat162 sum = nought;      // 0 x of all of them: a NaN where one is not finite
+#pragma unroll 4
+          for (int i = at0; i < unit_bytes / 16; i += STEP) {
+            const uint4 x = *reinterpret_cast<const uint4*>(v_s + 16 * i);
+            sum = __hfma2(reinterpret_cast<const __nv_bfloat162&>(x.x), nought, sum);
+            sum = __hfma2(reinterpret_cast<const __nv_bfloat162&>(x.y), nought, sum);
+            sum = __hfma2(reinterpret_cast<const __nv_bfloat162&>(x.z), nought, sum);
+            sum = __hfma2(reinterpret_cast<const __nv_bfloat162&>(x.w), nought, sum);
           }
-          if (any) spoiled[it & 1] = it + 1;
+          if (__low2float(sum) != 0.f || __high2float(sum) != 0.f) {
+            for (int i = at0; i < unit_bytes / 16; i += STEP) {
+              uint4 x = *reinterpret_cast<const uint4*>(v_s + 16 * i);
+              uint32_t* w4 = &x.x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w4[e] &= ~__vcmpeq2(w4[e] & 0x7f807f80u, 0x7f807f80u);
+              *reinterpret_cast<uint4*>(v_s + 16 * i) = x;
+            }
+            spoiled[it & 1] = it + 1;
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          asm volatile("bar.sync 5, 256;" ::: "memory");
+          if constexpr (KEYS) {
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + set), "n"(BM) : "memory");      // the tile is this set's alone
+          } else {
+            sync_softmax();
+          }
         }
         if (busy) {
-          constexpr int N = W < 64 ? W : 64;      // columns that a thread has in registers
-          auto shape = [&](float (&v)[N], int col) {
+          float v[N];
+          auto scores_at = [&](int col) {      // of this thread's columns col .. col + N - 1, -infinity where the row may not see the key
+            tmem_ld(v, s_addr + col);
             if (a.softcap > 0.f) {
 #pragma unroll
               for (int e = 0; e < N; ++e) v[e] = mi::shaped_logit2(v[e], a.scale, a.softcap, false, 0.f);
             }
             if (masked) {
 #pragma unroll
-              for (int e0 = 0; e0 < N; e0 += 32) {
-                const uint32_t bits = seen_bits(a, p.it, key0 + col + e0, begin, mask);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e0 + e] = (bits >> e) & 1 ? v[e0 + e] : -INFINITY;
-              }
+              for (int e = 0; e < N; ++e) v[e] = (bits[(col + e) / 32] >> (e & 31)) & 1 ? v[e] : -INFINITY;
             }
           };
-          auto largest = [&](const float (&v)[N]) {
+          auto largest = [&]() {
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int e = 0; e < N; e += 2) mx4[e >> 1 & 3] = mi::max_of(mx4[e >> 1 & 3], v[e], v[e + 1]);
             return fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
           };
-          float v[N], mx;
-          if constexpr (QT == 1) {
-            tmem_ld(v, s_addr + W * half);
-            shape(v, W * half);
-            float* maxima = row_max + (g & 1) * 2 * BM;
-            mx = largest(v);
-            maxima[half * BM + r] = mx;
-            tc_fence_before();
-            meet();      // both halves of the scores are in registers: the weights may be written over them
-            tc_fence_after();
-            mx = fmaxf(mx, maxima[(half ^ 1) * BM + r]);
-          } else {      // the second half of the scores stays in registers, the first is read again: the weights lie over the second
-            tmem_ld(v, s_addr);
-            shape(v, 0);
-            mx = largest(v);
-            tmem_ld(v, s_addr + 64);
-            shape(v, 64);
-            mx = fmaxf(mx, largest(v));
+          scores_at(0);
+          float mx = largest();
+          if constexpr (BN > N) {
+            scores_at(N);
+            mx = fmaxf(mx, largest());
           }
           const float m_new = fmaxf(m_run, mx * factor);      // the scale is positive
-          const bool move = m_new > m_run;
+          const bool move = m_new > m_run + 8.f;      // (of the first key: from -infinity)
           if (__any_sync(0xffffffffu, move)) {
             const float alpha = move ? exp2f(m_run - m_new) : 1.f;
-            if (j > 0) {
-              wait_o(g - 1);
+            if (!first_of_set) {      // (its last P V is done: this tile's scores came behind it)
 #pragma unroll 1
-              for (int c = half; 32 * c < k.n_out; c += HALVES) {
-                float o[32];
-                uint32_t x[32];
-                tmem_ld(o, o_addr + 32 * c);
+              for (int c = 0; 16 * c < k.n_out; ++c) {      // (16 at a time: the scores are in registers too)
+                float o[16];
+                uint32_t x[16];
+                tmem_ld(o, o_addr + 16 * c);
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
+                for (int e = 0; e < 16; e += 2) {
                   mi::mul_pair(o[e], o[e + 1], o[e], o[e + 1], alpha);
                   x[e] = __float_as_uint(o[e]);
                   x[e + 1] = __float_as_uint(o[e + 1]);
                 }
-                tmem_st(o_addr + 32 * c, x);
+                tmem_st(o_addr + 16 * c, x);
               }
             }
             l_run *= alpha;
@@ -615,63 +708,81 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
           }
           const float m_use = m_run == -INFINITY ? 0.f : m_run;
           float part[4] = {0.f, 0.f, 0.f, 0.f};
-          auto weigh = [&](float (&v)[N], uint32_t to) {      // two keys to a column
+          auto weigh = [&](int col) {      // over its own scores, two keys to a column
             uint32_t packed[N / 2];
 #pragma unroll
             for (int e = 0; e < N; e += 2) mi::fma_pair(v[e], v[e + 1], v[e], v[e + 1], factor, -m_use);
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
-              packed[e] = pack_bf16(mi::ex2_fast(v[2 * e]), mi::ex2_fast(v[2 * e + 1]));      // nothing where the row may not see the key
+              if (e % CUBIC_OF < CUBIC) {
+                ex2_cubic(v[2 * e], v[2 * e + 1]);
+              } else {
+                v[2 * e] = mi::ex2_fast(v[2 * e]);
+                v[2 * e + 1] = mi::ex2_fast(v[2 * e + 1]);
+              }
+              packed[e] = pack_bf16(v[2 * e], v[2 * e + 1]);      // nothing where the row may not see the key
               mi::add_pair(part[2 * e & 3], part[(2 * e + 1) & 3], __uint_as_float(packed[e] << 16), __uint_as_float(packed[e] & 0xffff0000u));
             }
-            tmem_st(to, packed);
+            tmem_st(s_addr + col, packed);
           };
-          if constexpr (QT == 1) {
-            weigh(v, s_addr + W / 2 * half);
-          } else {
-            weigh(v, s_addr + 96);
-            tmem_ld(v, s_addr);
-            shape(v, 0);
-            weigh(v, s_addr + 64);
+          weigh(BN - N);      // the last scores are still in registers, the first are read again
+          if constexpr (BN > N) {
+            scores_at(0);
+            weigh(0);
           }
           l_run += (part[0] + part[1]) + (part[2] + part[3]);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
-        if (g >= LAG) wait_o(g - LAG);      // long done: keeps this thread in step with the barrier
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
+        if (lane == 0) mbar_arrive(&p_full[set]);
       }
-#pragma unroll
-      for (int back = LAG; back > 0; --back)
-        if (g >= back) wait_o(g - back);
-      const bool whole = p.whole;
+      const bool whole = p.slot < 0, mine = !KEYS || set < tiles;      // (a piece of one tile has no second stream)
+      if (mine) {
+        mbar_wait(&o_full[set], (g - 1) & 1, abort, k.status);
+        tc_fence_after();
+      }
+      if (!(l_run < 1e30f)) l_run = __int_as_float(0x7fffffff);      // a score that is no number (ex2_cubic makes a huge weight of it)
+      float m_all = m_run, l_all = l_run, scale0 = 1.f, scale1 = 0.f;
+      if constexpr (KEYS) {      // the two streams' sums of this row
+        of_set[set * BM + r] = make_float2(m_run, l_run);
+        tc_fence_before();
+        sync_softmax();
+        tc_fence_after();
+        const float2 x0 = of_set[r], x1 = of_set[BM + r];
+        m_all = fmaxf(x0.x, x1.x);
+        const float off = m_all == -INFINITY ? 0.f : m_all;
+        scale0 = exp2f(x0.x - off);
+        scale1 = exp2f(x1.x - off);
+        l_all = x0.y * scale0 + x1.y * scale1;
+      }
       const bool fix = spoiled[it & 1] == it + 1;
-      float l_all = l_run;
-      if constexpr (QT == 1) {
-        row_sum[half * BM + r] = l_run;
-        meet();
-        l_all = row_sum[r] + row_sum[BM + r];
-      }
       const int h = p.head * a.G + r % a.G;
-      float mult = 1.f;
       if (whole) {
         const float sink2 = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
-        const float top = fmaxf(m_run, sink2), off = top == -INFINITY ? 0.f : top, weight = exp2f(m_run - off);
-        const float total = l_all * weight + exp2f(sink2 - off);
-        mult = total == 0.f ? 0.f : weight / total;      // nothing visible: zeros
+        const float top = fmaxf(m_all, sink2), off = top == -INFINITY ? 0.f : top, weight = exp2f(m_all - off);
+        const float total = l_all * weight + exp2f(sink2 - off), mult = total == 0.f ? 0.f : weight / total;      // nothing visible: zeros
+        scale0 *= mult;
+        scale1 *= mult;
       }
-      const int key_end = min(p.it.ctx, (p.l.t_begin + p.j0 + p.n) * BN);
-      const size_t at = (size_t)p.slot * (QT * BM) + set * BM + r;      // row of the sums
+      const int key_end = min(p.it.ctx, p.key + tiles * BN);
       if (busy) {
 #pragma unroll 1
-        for (int c = half; 32 * c < k.n_out; c += HALVES) {
+        for (int c = KEYS ? set : 0; 32 * c < k.n_out; c += KEYS ? 2 : 1) {
           float o[32];
-          tmem_ld(o, o_addr + 32 * c);
+          tmem_ld(o, (KEYS ? t_lane : o_addr) + 32 * c);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= scale0;
+          if (KEYS && tiles > 1) {
+            float o1[32];
+            tmem_ld(o1, t_lane + 128 + 32 * c);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(o1[e], scale1, o[e]);
+          }
           if (valid && !*abort) {
             if (fix) {
               float more[32] = {};
-              add_not_finite(a, p.it, p.head, touched, key_end, begin, mask, 32 * c, more);
+              add_not_finite(a, p.it, p.head, p.key, key_end, begin, mask, near, 32 * c, more);
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] += more[e];
             }
@@ -679,39 +790,23 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
               __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.nh * a.hd + (size_t)h * a.hd + 32 * c;
 #pragma unroll
               for (int q = 0; q < 4; ++q)
-                if (32 * c + 8 * q < a.hd) {      // (a head size is a multiple of 16)
-                  uint32_t x[4];
+                if (32 * c + 8 * q < a.hd)      // (a head size is a multiple of 16)
+                  *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(pack_bf16(o[8 * q], o[8 * q + 1]), pack_bf16(o[8 * q + 2], o[8 * q + 3]),
+                                                                      pack_bf16(o[8 * q + 4], o[8 * q + 5]), pack_bf16(o[8 * q + 6], o[8 * q + 7]));
+            } else {      // four columns of all rows, then the next four: what a warp's lanes write lies side by side
+              float4* dst = reinterpret_cast<float4*>(a.part_o) + ((size_t)p.slot * (k.n_out / 4) + 8 * c) * (QT * BM) + rows_set * BM + r;
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) x[e] = pack_bf16(o[8 * q + 2 * e] * mult, o[8 * q + 2 * e + 1] * mult);
-                  *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(x[0], x[1], x[2], x[3]);
-                }
-            } else {
-              float* dst = a.part_o + at * a.hd + 32 * c;
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                if (32 * c + 4 * q < a.hd) *reinterpret_cast<float4*>(dst + 4 * q) = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+              for (int q = 0; q < 8; ++q) dst[q * (QT * BM)] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
             }
           }
           __syncwarp();
         }
-        if (!whole && valid && half == 0 && !*abort) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(m_run, l_all);
-      }
-      if (threadIdx.x == 0 && p.j0 == 0) {      // the unit's pieces, for the kernel that joins them
-        const int blocks = start->blocks, me = (int)blockIdx.x;
-        const long long total = start->total, g_last = stretch_begin(total, me, blocks) + (start->left - walk.left) - p.n + p.l.tiles - 1;
-        int last = me;
-        if (!whole) {      // the block whose stretch holds the unit's last tile
-          last = (int)(g_last * blocks / total);
-          while (last + 1 < blocks && stretch_begin(total, last + 1, blocks) <= g_last) ++last;
-        }
-        k.units[((size_t)p.b * a.nkv + p.head) * k.max_parts + p.part] = make_int2(me, last - me + 1);
+        if (!whole && valid && (!KEYS || set == 0) && !*abort) reinterpret_cast<float2*>(a.part_ml)[(size_t)p.slot * (QT * BM) + rows_set * BM + r] = make_float2(m_all, l_all);
       }
       tc_fence_before();
-      meet();      // (the sums are read too: the next piece may leave its own)
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
-      u0 += 2 * p.n;
-      ++it;
+      u0 = (u0 + 2 * tiles) % (2 * k.ring);      // (as far as slot and parity go)
     }
   }
   // every tensor-memory access is done, then the columns go back
@@ -724,63 +819,69 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
   }
 }
 
-// The pieces of units that several blocks shared, added up: grid (items * nkv * max_parts, rows / JOIN_WARPS), a warp a row, four values a lane.
+// The pieces of units that several blocks shared, added up: for the unit that begins in a block and goes on in others, grid (blocks, QT, columns / (4 F
+// JOIN_WARPS / 4)); a lane a row and 4 F columns, a warp 32 rows.  Piece s lies in block first + s: as that block's second of the sums where the unit
+// begins there, else as its first.  AT_ONCE pieces are on their way at a time, their maxima and sums with them.
 constexpr int JOIN_WARPS = 8;
-template <int QT>
+template <int QT, int F, int AT_ONCE>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
 tree_join_kernel(const Tc k) {
   const Args& a = k.a;
-  const int unit = blockIdx.x, part = unit % k.max_parts, head = unit / k.max_parts % a.nkv, b = unit / k.max_parts / a.nkv;
-  const int row = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;      // of the unit's QT * 128
+  const int warp = threadIdx.x >> 5, set = blockIdx.y, r = warp % 4 * 32 + (threadIdx.x & 31), f0 = (blockIdx.z * (JOIN_WARPS / 4) + warp / 4) * F, row = set * BM + r;
   mi::grid_dependency_sync();
-  const Item it = item_of(a, b);
-  const int set = row / BM, r = row - set * BM, first = (part * QT + set) * k.tokens;
-  if (r >= min(k.tokens, it.n - first) * a.G) return;
-  const int2 u = k.units[unit];
-  const int pieces = u.y;
-  if (pieces <= 1) return;
-  // piece s lies in block u.x + s: its first piece where the unit begins there, else the one that its stretch begins with
-  auto slot = [&](int s) { return (size_t)(2 * (u.x + s) + (s == 0 ? 1 : 0)) * (QT * BM) + row; };
-  const int h = head * a.G + r % a.G;
+  const int4 u = k.joins[blockIdx.x];
+  const int first = (int)blockIdx.x, pieces = u.x, token = u.y + set * k.tokens + r / a.G, h = u.w * a.G + r % a.G;
+  if (pieces == 0 || r >= min(k.tokens, u.z - set * k.tokens) * a.G || 4 * f0 >= a.hd) return;
+  const float2* sums = reinterpret_cast<const float2*>(a.part_ml) + row;
+  const float4* values = reinterpret_cast<const float4*>(a.part_o) + (size_t)f0 * (QT * BM) + row;
   const float sink2 = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
-  float2 mine = make_float2(-INFINITY, 0.f);
-  if (lane < pieces) mine = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(lane));
-  float top = fmaxf(mine.x, sink2);
-  for (int s = 32 + lane; s < pieces; s += 32) top = fmaxf(top, a.part_ml[2 * slot(s)]);
-  top = mi::warp_max(top);
-  const float off = top == -INFINITY ? 0.f : top;
-  float f = exp2f(mine.x - off), total = mine.y * f;
-  float acc[2][4] = {};
+  float top = sink2, total = a.sink ? 1.f : 0.f;
+  float acc[F][4] = {};
 #pragma unroll 1
-  for (int s0 = 0; s0 < pieces; s0 += 32) {
-    if (s0 > 0) {
-      mine = s0 + lane < pieces ? *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(s0 + lane)) : make_float2(-INFINITY, 0.f);
-      f = exp2f(mine.x - off);
-      total += mine.y * f;
-    }
-    const int near = min(32, pieces - s0);
-#pragma unroll 4
-    for (int s = 0; s < near; ++s) {
-      const float w = __shfl_sync(0xffffffffu, f, s);
-      const float* src = a.part_o + slot(s0 + s) * a.hd;
+  for (int s0 = 0; s0 < pieces; s0 += AT_ONCE) {
+    float2 ml[AT_ONCE];
+    float4 x[AT_ONCE][F];
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (128 * c + 4 * lane < a.hd) {
-          const float4 x = *reinterpret_cast<const float4*>(src + 128 * c + 4 * lane);
-          acc[c][0] = fmaf(x.x, w, acc[c][0]);
-          acc[c][1] = fmaf(x.y, w, acc[c][1]);
-          acc[c][2] = fmaf(x.z, w, acc[c][2]);
-          acc[c][3] = fmaf(x.w, w, acc[c][3]);
-        }
+    for (int s = 0; s < AT_ONCE; ++s) {
+      ml[s] = make_float2(-INFINITY, 0.f);
+      const size_t at = 2 * (first + s0 + s) + (s0 + s == 0 ? 1 : 0);
+      if (s0 + s < pieces) ml[s] = sums[at * (QT * BM)];
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        x[s][f] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s0 + s < pieces) x[s][f] = values[(at * (k.n_out / 4) + f) * (QT * BM)];
+      }
+    }
+    float next = top;
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s) next = fmaxf(next, ml[s].x);
+    const float off = next == -INFINITY ? 0.f : next, alpha = exp2f(top - off);
+    top = next;
+    total *= alpha;
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[f][e] *= alpha;
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s) {
+      const float w = exp2f(ml[s].x - off);
+      total = fmaf(ml[s].y, w, total);
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        acc[f][0] = fmaf(x[s][f].x, w, acc[f][0]);
+        acc[f][1] = fmaf(x[s][f].y, w, acc[f][1]);
+        acc[f][2] = fmaf(x[s][f].z, w, acc[f][2]);
+        acc[f][3] = fmaf(x[s][f].w, w, acc[f][3]);
+      }
     }
   }
-  total = mi::warp_sum(total) + exp2f(sink2 - off);
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)(it.row0 + first + r / a.G) * a.nh + h) * a.hd;
+  const float inv = total == 0.f ? 0.f : 1.f / total;      // nothing visible: zeros
+  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)token * a.nh + h) * a.hd + 4 * f0;
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
-    if (128 * c + 4 * lane < a.hd)
-      *reinterpret_cast<uint2*>(dst + 128 * c + 4 * lane) = make_uint2(pack_bf16(acc[c][0] * inv, acc[c][1] * inv), pack_bf16(acc[c][2] * inv, acc[c][3] * inv));
+  for (int f = 0; f < F; f += 2)      // (a head size is a multiple of 16)
+    if (4 * (f0 + f) < a.hd)
+      *reinterpret_cast<uint4*>(dst + 4 * f) = make_uint4(pack_bf16(acc[f][0] * inv, acc[f][1] * inv), pack_bf16(acc[f][2] * inv, acc[f][3] * inv),
+                                                          pack_bf16(acc[f + 1][0] * inv, acc[f + 1][1] * inv), pack_bf16(acc[f + 1][2] * inv, acc[f + 1][3] * inv));
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -795,25 +896,27 @@ EncodeFn encoder() {
   return fn;
 }
 
-template <int QT, int BN>
+template <int QT, int SETS, int BN, int STEPS>
 int launch(Tc& k, const CUtensorMap& q_map, const CUtensorMap& kv_map, int blocks, cudaStream_t stream) {
   static bool ready[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return mi_fail("attention_tree_tc: no current device");
   if (!ready[dev]) {
-    if (cudaFuncSetAttribute(tree_tc_kernel<QT, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
+    if (cudaFuncSetAttribute(tree_tc_kernel<QT, SETS, BN, STEPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
       return mi_fail("attention_tree_tc: %d bytes of shared memory were refused", SMEM_BYTES);
     ready[dev] = true;
   }
-  k.ring = (SMEM_BYTES - 1024 - SMEM_TAIL - QT * k.boxes * BM * 128) / (k.boxes * BN * 128);
+  k.ring = (SMEM_BYTES - BARS * 8 - (QT == 1 ? 2 * BM * 8 : 0) - QT * k.boxes * BM * 128) / (k.boxes * BN * 128);
   if (k.ring > MAX_UNITS) k.ring = MAX_UNITS;
   MI_REQUIRE(k.ring >= 4, "attention_tree_tc: no room for a ring of tiles of %d boxes", k.boxes);
-  if (mi::launch(tree_tc_kernel<QT, BN>, dim3(blocks), dim3(THREADS), SMEM_BYTES, stream, q_map, kv_map, k) != cudaSuccess)
+  if (mi::launch(tree_tc_kernel<QT, SETS, BN, STEPS>, dim3(blocks), dim3(threads_of(SETS)), SMEM_BYTES, stream, q_map, kv_map, k) != cudaSuccess)
     return mi_fail("attention_tree_tc: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  // Many pieces of a unit where there are fewer units than blocks: eight at a time of 8 columns; else two at a time of 32.
   const Args& a = k.a;
-  const int rows = a.max_q * a.G < QT * BM ? a.max_q * a.G : QT * BM;      // (a set's last rows may be empty: groups that do not divide 128)
-  const int join_rows = QT == 2 && rows > BM ? QT * BM : rows;
-  if (mi::launch(tree_join_kernel<QT>, dim3(a.items * a.nkv * k.max_parts, (join_rows + JOIN_WARPS - 1) / JOIN_WARPS), dim3(32 * JOIN_WARPS), 0, stream, k) != cudaSuccess)
+  const bool few = (long long)a.items * a.nkv * k.max_parts < blocks;
+  const int f = few ? 2 : 8, columns = (k.n_out / 4 + f * (JOIN_WARPS / 4) - 1) / (f * (JOIN_WARPS / 4));
+  auto join = few ? tree_join_kernel<QT, 2, 8> : tree_join_kernel<QT, 8, 2>;
+  if (mi::launch(join, dim3(blocks, QT, columns), dim3(32 * JOIN_WARPS), 0, stream, k) != cudaSuccess)
     return mi_fail("attention_tree_tc: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   MI_LAUNCH_OK("attention_tree_tc");
   return 0;
@@ -825,23 +928,24 @@ int sets_of(int max_q, int G, int hd) { return hd <= 128 && max_q > BM / G ? 2 :
 }  // namespace
 
 // Whether the kernel takes these sizes and addresses.
-MI_API int mi_attention_tree_tc_takes(const void* out, const void* qkv, const void* kv, int T, int width, int nh, int nkv, int hd, long long pages, int page_size, int max_q, float scale) {
+MI_API int mi_attention_tree_tc_takes(const void* out, const void* qkv, const void* kv, int items, int bt_stride, int T, int width, int nh, int nkv, int hd, long long pages, int page_size, int max_q, float scale) {
   return nkv > 0 && nh % nkv == 0 && nh / nkv <= BM && hd % 16 == 0 && hd >= 64 && hd <= 256 && width % 8 == 0 && page_size % 16 == 0 && scale > 0.f && T > 0 &&
-         (((uintptr_t)out | (uintptr_t)qkv | (uintptr_t)kv) % 16) == 0 && pages * 2 * nkv * page_size <= 0x7fffffffll && max_q > 0;
+         (((uintptr_t)out | (uintptr_t)qkv | (uintptr_t)kv) % 16) == 0 && pages * 2 * nkv * page_size <= 0x7fffffffll && max_q > 0 &&
+         ((long long)bt_stride * page_size / 64 + 2 + OVERHEAD) * items * nkv * (max_q / (BM / (nh / nkv)) + 1) <= 0x7fffffffll;      // the line of tiles
 }
-// Floats of scratch: the units' pieces, the sums.
-MI_API long long mi_attention_tree_tc_floats(int items, int nh, int nkv, int hd, int max_q) {
-  const int G = nh / nkv, qt = sets_of(max_q, G, hd), tokens = BM / G, parts = (max_q + qt * tokens - 1) / (qt * tokens);
-  return 4ll * items * nkv * parts + 2ll * mi::sm_count() * qt * BM * (hd + 2);
+// Floats of scratch: what is to be joined, the sums.
+MI_API long long mi_attention_tree_tc_floats(int nh, int nkv, int hd, int max_q) {
+  const long long blocks = mi::sm_count();
+  return 4 * blocks + 2 * blocks * sets_of(max_q, nh / nkv, hd) * BM * ((hd + BOX - 1) / BOX * BOX + 2);
 }
 
 // bfloat16, what mi_attention_tree_tc_takes says.  scratch: mi_attention_tree_tc_floats floats, 16-byte aligned; status: one word, set to 2 if a
-// bounded wait ran out.
+// bounded wait ran out, to 4 if shared memory is not laid out as the kernel needs it.
 MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, const int* block_table, int bt_stride, const int* q_start, const int* q_len,
                                 const int* ctx_len, const int* seq_slot, const int* mask, int words, const int* positions, const float* sink, float* scratch,
                                 int* status, int items, int T, int width, int nh, int nkv, int hd, int pages, int page_size, int window, int max_q, float scale,
                                 float softcap, cudaStream_t stream) {
-  MI_REQUIRE(mi_attention_tree_tc_takes(out, qkv, kv, T, width, nh, nkv, hd, pages, page_size, max_q, scale), "attention_tree_tc: sizes or addresses that it does not take");
+  MI_REQUIRE(mi_attention_tree_tc_takes(out, qkv, kv, items, bt_stride, T, width, nh, nkv, hd, pages, page_size, max_q, scale), "attention_tree_tc: sizes or addresses that it does not take");
   MI_REQUIRE(items >= 0 && bt_stride > 0 && pages > 0 && (long long)words * 32 >= max_q && ((uintptr_t)scratch % 16) == 0, "attention_tree_tc: bad sizes items=%d words=%d max_q=%d", items, words, max_q);
   if (items == 0) return 0;
   const EncodeFn encode = encoder();
@@ -856,12 +960,10 @@ MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, cons
   k.tokens = BM / G;
   k.max_parts = (max_q + qt * k.tokens - 1) / (qt * k.tokens);
   k.scale_log2 = scale * 1.4426950408889634f;
-  const long long units = (long long)items * nkv * k.max_parts;
-  MI_REQUIRE(units <= 0x7fffffffll, "attention_tree_tc: %d items of %d heads in %d parts are too many", items, nkv, k.max_parts);
   const int blocks = mi::sm_count();
-  k.units = (int2*)scratch;
-  float* part_o = scratch + 4 * units;
-  float* part_ml = part_o + 2ll * blocks * qt * BM * hd;
+  k.joins = (int4*)scratch;
+  float* part_o = scratch + 4ll * blocks;
+  float* part_ml = part_o + 2ll * blocks * qt * BM * k.n_out;
   k.a = Args{out, qkv, kv, block_table, bt_stride, q_start, q_len, ctx_len, seq_slot, mask, words, positions, sink, part_o, part_ml,
              items, T, width, nh, nkv, G, hd, pages, page_size, window, max_q, scale, softcap};
   CUtensorMap q_map, kv_map;
@@ -879,6 +981,12 @@ MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, cons
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return mi_fail("attention_tree_tc: cuTensorMapEncodeTiled of the cache failed with code %d", (int)r);
   }
-  if (qt == 2) return launch<2, 128>(k, q_map, kv_map, blocks, stream);
-  return hd <= 128 ? launch<1, 128>(k, q_map, kv_map, blocks, stream) : launch<1, 64>(k, q_map, kv_map, blocks, stream);
+  // heads of 64, 128 and 256 with the products' steps written out
+  if (qt == 2) {
+    if (hd == 128) return launch<2, 2, 128, 8>(k, q_map, kv_map, blocks, stream);
+    return hd == 64 ? launch<2, 2, 128, 4>(k, q_map, kv_map, blocks, stream) : launch<2, 2, 128, 0>(k, q_map, kv_map, blocks, stream);
+  }
+  if (hd == 128) return launch<1, 2, 128, 8>(k, q_map, kv_map, blocks, stream);
+  if (hd < 128) return hd == 64 ? launch<1, 2, 128, 4>(k, q_map, kv_map, blocks, stream) : launch<1, 2, 128, 0>(k, q_map, kv_map, blocks, stream);
+  return hd == 256 ? launch<1, 1, 64, 16>(k, q_map, kv_map, blocks, stream) : launch<1, 1, 64, 0>(k, q_map, kv_map, blocks, stream);
 }

@@ -1670,10 +1670,11 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
            _ptr(batch.positions if win else None, torch.int32), _ptr(sink))
   sizes = (batch.num_items, T, qkv.shape[1], num_heads, num_kv_heads, head_dim, kv_layer.shape[0], page_size, win, int(batch.max_q_len),
            ctypes.c_float(scale), ctypes.c_float(softcap))
-  if dt == BF16 and lib.mi_attention_tree_tc_takes(_ptr(out), _ptr(qkv), _ptr(kv_layer), T, qkv.shape[1], num_heads, num_kv_heads, head_dim,
-                                                   ctypes.c_longlong(kv_layer.shape[0]), page_size, int(batch.max_q_len), ctypes.c_float(scale)):
+  if dt == BF16 and lib.mi_attention_tree_tc_takes(_ptr(out), _ptr(qkv), _ptr(kv_layer), batch.num_items, block_table.shape[1], T, qkv.shape[1],
+                                                   num_heads, num_kv_heads, head_dim, ctypes.c_longlong(kv_layer.shape[0]), page_size, int(batch.max_q_len), ctypes.c_float(scale)):
+    shape = (batch.num_items, num_heads, num_kv_heads, head_dim, int(batch.max_q_len))
     lib.mi_attention_tree_tc_floats.restype = ctypes.c_longlong
-    n = int(lib.mi_attention_tree_tc_floats(batch.num_items, num_heads, num_kv_heads, head_dim, int(batch.max_q_len)))
+    n = int(lib.mi_attention_tree_tc_floats(num_heads, num_kv_heads, head_dim, int(batch.max_q_len)))
     if batch.scratch is not None:
       scratch, status = batch.scratch.buffer("attention_tree_partials", (n,), torch.float32), batch.scratch.zeros("attention_tree_status", 1, torch.int32)
     else:
