@@ -927,26 +927,24 @@ int sets_of(int max_q, int G, int hd) { return hd <= 128 && max_q > BM / G ? 2 :
 
 }  // namespace
 
-// Whether the kernel takes these sizes and addresses.
-MI_API int mi_attention_tree_tc_takes(const void* out, const void* qkv, const void* kv, int items, int bt_stride, int T, int width, int nh, int nkv, int hd, long long pages, int page_size, int max_q, float scale) {
-  return nkv > 0 && nh % nkv == 0 && nh / nkv <= BM && hd % 16 == 0 && hd >= 64 && hd <= 256 && width % 8 == 0 && page_size % 16 == 0 && scale > 0.f && T > 0 &&
-         (((uintptr_t)out | (uintptr_t)qkv | (uintptr_t)kv) % 16) == 0 && pages * 2 * nkv * page_size <= 0x7fffffffll && max_q > 0 &&
-         ((long long)bt_stride * page_size / 64 + 2 + OVERHEAD) * items * nkv * (max_q / (BM / (nh / nkv)) + 1) <= 0x7fffffffll;      // the line of tiles
-}
-// Floats of scratch: what is to be joined, the sums.
-MI_API long long mi_attention_tree_tc_floats(int nh, int nkv, int hd, int max_q) {
+// Floats of scratch - what is to be joined, the sums -, 0 for sizes that the kernel does not take.
+MI_API long long mi_attention_tree_tc_floats(int nh, int nkv, int hd, int page_size, int max_q) {
+  if (!(nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= BM && hd % 16 == 0 && hd >= 64 && hd <= 256 && page_size > 0 && page_size % 16 == 0 && max_q > 0)) return 0;
   const long long blocks = mi::sm_count();
   return 4 * blocks + 2 * blocks * sets_of(max_q, nh / nkv, hd) * BM * ((hd + BOX - 1) / BOX * BOX + 2);
 }
 
-// bfloat16, what mi_attention_tree_tc_takes says.  scratch: mi_attention_tree_tc_floats floats, 16-byte aligned; status: one word, set to 2 if a
-// bounded wait ran out, to 4 if shared memory is not laid out as the kernel needs it.
+// bfloat16.  scratch: mi_attention_tree_tc_floats floats, 16-byte aligned; status: one word, set to 2 if a bounded wait ran out, to 4 if shared memory is
+// not laid out as the kernel needs it.  Answers 2 for sizes or addresses that it does not take.
 MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, const int* block_table, int bt_stride, const int* q_start, const int* q_len,
                                 const int* ctx_len, const int* seq_slot, const int* mask, int words, const int* positions, const float* sink, float* scratch,
                                 int* status, int items, int T, int width, int nh, int nkv, int hd, int pages, int page_size, int window, int max_q, float scale,
                                 float softcap, cudaStream_t stream) {
-  MI_REQUIRE(mi_attention_tree_tc_takes(out, qkv, kv, items, bt_stride, T, width, nh, nkv, hd, pages, page_size, max_q, scale), "attention_tree_tc: sizes or addresses that it does not take");
-  MI_REQUIRE(items >= 0 && bt_stride > 0 && pages > 0 && (long long)words * 32 >= max_q && ((uintptr_t)scratch % 16) == 0, "attention_tree_tc: bad sizes items=%d words=%d max_q=%d", items, words, max_q);
+  MI_REQUIRE(items >= 0 && T >= 0 && nkv > 0 && nh % nkv == 0 && bt_stride > 0 && pages > 0 && (long long)words * 32 >= max_q, "attention_tree_tc: bad sizes items=%d T=%d words=%d max_q=%d", items, T, words, max_q);
+  if (mi_attention_tree_tc_floats(nh, nkv, hd, page_size, max_q) == 0 || width % 8 != 0 || !(scale > 0.f) || T == 0 ||
+      ((uintptr_t)out | (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)scratch) % 16 != 0 || (long long)pages * 2 * nkv * page_size > 0x7fffffffll ||
+      ((long long)bt_stride * page_size / 64 + 2 + OVERHEAD) * items * nkv * (max_q / (BM / (nh / nkv)) + 1) > 0x7fffffffll)      // the last: the line of tiles
+    return 2;
   if (items == 0) return 0;
   const EncodeFn encode = encoder();
   if (!encode) return mi_fail("attention_tree_tc: the driver does not offer cuTensorMapEncodeTiled");

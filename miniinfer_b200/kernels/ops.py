@@ -1325,18 +1325,40 @@ def sample(out: torch.Tensor, logits: torch.Tensor, temperature: torch.Tensor, t
                             _stream()), kernels=2)
 
 
-def _here(t: torch.Tensor, what: str) -> None:
-  """Refuses a tensor that is not on the current device, whose stream the launch goes to."""
+_C_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+_entries: Dict[str, ctypes._CFuncPtr] = {}
+
+
+def _entry(name: str, arguments: str, result: str = "i"):
+  """An exported function of the common library with its arguments' types declared, a letter each: plain numbers and addresses then go over
+  without an object made for each (a call of thirty arguments: 4 us instead of 15)."""
+  f = _entries.get(name)
+  if f is None:
+    f = getattr(common_lib(), name)
+    f.argtypes, f.restype = [_C_TYPES[c] for c in arguments], _C_TYPES[result]
+    _entries[name] = f
+  return f
+
+
+def _device(what: str, t: torch.Tensor) -> int:
+  """The index of the tensor's device; refuses a tensor that is not on the current device, whose stream the launch goes to."""
   if not t.is_cuda:
     raise KernelError("the engine's kernels run on CUDA tensors only (got a CPU tensor)")
-  if t.device.index != torch.cuda.current_device():
-    raise KernelError(f"{what}: the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+  device = t.get_device()
+  if device != torch.cuda.current_device():
+    raise KernelError(f"{what}: the tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+  return device
 
 
-def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-  for t in others:
-    if t is not None and t.device != first.device:
-      raise KernelError(f"{what}: the tensors are on several devices ({first.device}, {t.device})")
+def _address(what: str, t: torch.Tensor, dtype: torch.dtype, device: int) -> int:
+  if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+    raise KernelError(f"{what}: expected a contiguous tensor of {dtype} on cuda:{device}, got {t.dtype} on {t.device}"
+                      + ("" if t.is_contiguous() else ", not contiguous"))
+  return t.data_ptr()
+
+
+def _current_stream(device: int) -> int:
+  return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 BEAM_MAX_BEST = 128     # the most places of a request that one selection fills
@@ -1363,49 +1385,50 @@ def beam_select(tokens: torch.Tensor, parents: torch.Tensor, scores: torch.Tenso
   dt = _dt(logits)
   if requests == 0:
     return
-  _same_device("beam_select", logits, tokens, parents, scores, cum, row_start)
-  _here(logits, "beam_select")
-  lib = common_lib()
-  lib.mi_beam_select_words.restype = ctypes.c_longlong
-  words = int(lib.mi_beam_select_words(R, V, n))
+  device = _device("beam_select", logits)
+  at = lambda t, dtype: _address("beam_select", t, dtype, device)      # noqa: E731
+  words = int(_entry("mi_beam_select_words", "iii", "l")(R, V, n))
   if workspace is not None:
-    scratch = workspace.buffer("beam_scratch", (max(words, 1),), torch.int64)
+    scratch = workspace.buffer("beam_scratch", (words,), torch.int64)
     arrivals = workspace.zeros("beam_arrivals", requests, torch.int32)
   else:
-    scratch = torch.empty(max(words, 1), dtype=torch.int64, device=logits.device)
+    scratch = torch.empty(words, dtype=torch.int64, device=logits.device)
     arrivals = torch.zeros(requests, dtype=torch.int32, device=logits.device)
-  _check(lib, lib.mi_beam_select(_ptr(tokens, torch.int32), _ptr(parents, torch.int32), _ptr(scores, torch.float32), _ptr(logits), dt,
-                                 _ptr(cum, torch.float32), _ptr(row_start, torch.int32), _ptr(scratch), _ptr(arrivals), R, V, requests, n,
-                                 _stream()))
+  _check(common_lib(), _entry("mi_beam_select", "ppppipppp" + "iiiip")(
+    at(tokens, torch.int32), at(parents, torch.int32), at(scores, torch.float32), at(logits, logits.dtype), dt, at(cum, torch.float32),
+    at(row_start, torch.int32), at(scratch, torch.int64), at(arrivals, torch.int32), R, V, requests, n, _current_stream(device)))
 
 
 MOVE_MAX_PAIRS = 4096   # the most pairs of one call of reorder_states or copy_cache_pages
 
 
-def _pairs(what: str, base: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *more: Optional[torch.Tensor]) -> int:
+def _pairs(what: str, src: torch.Tensor, dst: torch.Tensor) -> int:
   if src.dim() != 1 or src.shape != dst.shape:
     raise KernelError(f"{what}: sources and destinations must be two lists of one length")
-  _same_device(what, base, src, dst, *more)
   return src.shape[0]
+
+
+def _move_places(what: str, base: torch.Tensor, layers: int, places: int, place_bytes: int, src, dst, filled, page: int, token_bytes: int, n: int) -> None:
+  if n > MOVE_MAX_PAIRS:
+    raise KernelError(f"{what}: {n} pairs, at most {MOVE_MAX_PAIRS} go in one call")
+  if n == 0 or base.numel() == 0:
+    return
+  device = _device(what, base)
+  at = lambda t: _address(what, t, torch.int32, device)      # noqa: E731
+  _check(common_lib(), _entry("mi_move_places", "pillpppi" + "lip")(base.data_ptr(), layers, places, place_bytes, at(src), at(dst), at(filled) if filled is not None else 0,
+                                                              page, token_bytes, n, _current_stream(device)))
 
 
 def reorder_states(state: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
   """``state[:, dst[k]] = state[:, src[k]]`` for a group's per-request states ``[layers, slots, ...]`` of any type, as if every source were
   read before any destination is written: the beams of a request may change places.  ``src``, ``dst`` int32 ``[pairs]``, at most
   ``MOVE_MAX_PAIRS``; a pair with an index out of range is left out (padding: -1), the destinations differ from one another."""
-  n = _pairs("reorder_states", state, src, dst)
+  n = _pairs("reorder_states", src, dst)
   if state.dim() < 2 or not state.is_contiguous():
     raise KernelError("reorder_states: the states must be contiguous [layers, slots, ...]")
-  if n > MOVE_MAX_PAIRS:
-    raise KernelError(f"reorder_states: {n} pairs, at most {MOVE_MAX_PAIRS} go in one call")
-  if n == 0 or state.numel() == 0:
-    return
-  _here(state, "reorder_states")
-  lib = common_lib()
-  L, S = state.shape[:2]
-  none = ctypes.c_void_p(0)
-  _check(lib, lib.mi_move_places(_ptr(state), L, ctypes.c_longlong(S), ctypes.c_longlong(state.numel() // (L * S) * state.element_size()),
-                                 _ptr(src, torch.int32), _ptr(dst, torch.int32), none, 0, ctypes.c_longlong(0), n, _stream()))
+  layers, slots = state.shape[:2]
+  bytes_of_slot = state.numel() // (layers * slots) * state.element_size() if state.numel() else 0
+  _move_places("reorder_states", state, layers, slots, bytes_of_slot, src, dst, None, 0, 0, n)
 
 
 def copy_cache_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, filled: Optional[torch.Tensor] = None) -> None:
@@ -1413,21 +1436,14 @@ def copy_cache_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, fil
   with ``filled [pairs]`` int32 its first ``filled[k]`` tokens.  As if every source were read before any destination is written, so pages may
   also change places.  Indices int32, at most ``MOVE_MAX_PAIRS`` pairs; a pair with an index out of range is left out, the destinations
   differ from one another."""
-  n = _pairs("copy_cache_pages", kv, src, dst, filled)
+  n = _pairs("copy_cache_pages", src, dst)
   if kv.dim() != 6 or kv.shape[2] != 2 or not kv.is_contiguous():
     raise KernelError(f"copy_cache_pages: the pool must be contiguous [layers, pages, 2, heads, page_size, head_dim], got {tuple(kv.shape)}")
   if filled is not None and filled.shape != src.shape:
     raise KernelError("copy_cache_pages: one filled length for each pair")
-  if n > MOVE_MAX_PAIRS:
-    raise KernelError(f"copy_cache_pages: {n} pairs, at most {MOVE_MAX_PAIRS} go in one call")
-  if n == 0 or kv.numel() == 0:
-    return
-  _here(kv, "copy_cache_pages")
-  lib = common_lib()
-  L, pages, _, heads, P, hd = kv.shape
-  row = hd * kv.element_size()
-  _check(lib, lib.mi_move_places(_ptr(kv), L, ctypes.c_longlong(pages), ctypes.c_longlong(2 * heads * P * row), _ptr(src, torch.int32),
-                                 _ptr(dst, torch.int32), _ptr(filled, torch.int32), P, ctypes.c_longlong(row), n, _stream()))
+  layers, pages, _, heads, page, dim = kv.shape
+  row = dim * kv.element_size()
+  _move_places("copy_cache_pages", kv, layers, pages, 2 * heads * page * row, src, dst, filled, page, row, n)
 
 
 def move_cache_rows(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, group_start: torch.Tensor, most: int) -> None:
@@ -1437,18 +1453,19 @@ def move_cache_rows(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, grou
   were read before any of its destinations is written - ``most`` pairs at a time, in order, so ``most`` is at least a group's pairs, unless
   no destination lies behind its source -, while different groups touch different places.  All indices int32; a pair with an
   index out of range is left out, a group's destinations differ."""
-  n = _pairs("move_cache_rows", kv, src, dst, group_start)
+  n = _pairs("move_cache_rows", src, dst)
   if kv.dim() != 6 or kv.shape[2] != 2 or not kv.is_contiguous():
     raise KernelError(f"move_cache_rows: the pool must be contiguous [layers, pages, 2, heads, page_size, head_dim], got {tuple(kv.shape)}")
   if group_start.dim() != 1 or group_start.shape[0] < 1 or most < 1:
     raise KernelError("move_cache_rows: group_start must be [groups + 1], most at least 1")
-  if n == 0 or kv.numel() == 0 or group_start.shape[0] == 1:
+  groups = group_start.shape[0] - 1
+  if n == 0 or kv.numel() == 0 or groups == 0:
     return
-  _here(kv, "move_cache_rows")
-  lib = common_lib()
-  L, pages, _, heads, P, hd = kv.shape
-  _check(lib, lib.mi_move_cache_rows(_ptr(kv), L, ctypes.c_longlong(pages), heads, P, ctypes.c_longlong(hd * kv.element_size()), _ptr(src, torch.int32),
-                                     _ptr(dst, torch.int32), _ptr(group_start, torch.int32), n, group_start.shape[0] - 1, int(most), _stream()))
+  device = _device("move_cache_rows", kv)
+  at = lambda t: _address("move_cache_rows", t, torch.int32, device)      # noqa: E731
+  layers, pages, _, heads, page, dim = kv.shape
+  _check(common_lib(), _entry("mi_move_cache_rows", "piliil" + "pppiiip")(kv.data_ptr(), layers, pages, heads, page, dim * kv.element_size(), at(src), at(dst),
+                                                                    at(group_start), n, groups, int(most), _current_stream(device)))
 
 
 class AttentionBatch:
@@ -1661,39 +1678,54 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
   dt = _dt(qkv)
   if T == 0 or batch.num_items == 0 or batch.max_q_len <= 0:
     return
-  _same_device("tree_attention", qkv, out, kv_layer, block_table, mask, batch.q_start, batch.q_len, batch.ctx_len, batch.seq_slot, sink)
-  _here(qkv, "tree_attention")
-  lib = common_lib()
-  win, page_size = int(window or 0), kv_layer.shape[3]
-  where = (_ptr(block_table, torch.int32), block_table.shape[1], _ptr(batch.q_start, torch.int32), _ptr(batch.q_len, torch.int32),
-           _ptr(batch.ctx_len, torch.int32), _ptr(batch.seq_slot, torch.int32), _ptr(mask, torch.int32), mask.shape[1],
-           _ptr(batch.positions if win else None, torch.int32), _ptr(sink))
-  sizes = (batch.num_items, T, qkv.shape[1], num_heads, num_kv_heads, head_dim, kv_layer.shape[0], page_size, win, int(batch.max_q_len),
-           ctypes.c_float(scale), ctypes.c_float(softcap))
-  if dt == BF16 and lib.mi_attention_tree_tc_takes(_ptr(out), _ptr(qkv), _ptr(kv_layer), batch.num_items, block_table.shape[1], T, qkv.shape[1],
-                                                   num_heads, num_kv_heads, head_dim, ctypes.c_longlong(kv_layer.shape[0]), page_size, int(batch.max_q_len), ctypes.c_float(scale)):
-    shape = (batch.num_items, num_heads, num_kv_heads, head_dim, int(batch.max_q_len))
-    lib.mi_attention_tree_tc_floats.restype = ctypes.c_longlong
-    n = int(lib.mi_attention_tree_tc_floats(num_heads, num_kv_heads, head_dim, int(batch.max_q_len)))
-    if batch.scratch is not None:
-      scratch, status = batch.scratch.buffer("attention_tree_partials", (n,), torch.float32), batch.scratch.zeros("attention_tree_status", 1, torch.int32)
+  device = _device("tree_attention", qkv)
+  at = lambda t, dtype=torch.int32: _address("tree_attention", t, dtype, device)      # noqa: E731
+  win, page_size, max_q, ws = int(window or 0), kv_layer.shape[3], int(batch.max_q_len), batch.scratch
+  head = (at(out, qkv.dtype), at(qkv, qkv.dtype))
+  where = (at(kv_layer, qkv.dtype), at(block_table), block_table.shape[1], at(batch.q_start), at(batch.q_len), at(batch.ctx_len), at(batch.seq_slot),
+           at(mask), mask.shape[1], at(batch.positions) if win else 0, at(sink, torch.float32) if sink is not None else 0)
+  sizes = (batch.num_items, T, qkv.shape[1], num_heads, num_kv_heads, head_dim, kv_layer.shape[0], page_size, win, max_q, scale, softcap)
+  stream = _current_stream(device)
+  n = _tree_tc_floats(num_heads, num_kv_heads, head_dim, page_size, max_q) if dt == BF16 else 0
+  if n:
+    if ws is not None:
+      scratch, status = ws.buffer("attention_tree_partials", (n,), torch.float32), ws.zeros("attention_tree_status", 1, torch.int32)
     else:
-      scratch, status = torch.empty(n, dtype=torch.float32, device=qkv.device), torch.zeros(1, dtype=torch.int32, device=qkv.device)
-    _check(lib, lib.mi_attention_tree_tc(_ptr(out), _ptr(qkv), _ptr(kv_layer), *where, _ptr(scratch), _ptr(status), *sizes, _stream()), kernels=2)
-    if batch.scratch is None and int(status[0]) != 0:
-      raise KernelError("tree_attention: a bounded wait on a barrier ran out")
-    return
+      scratch = torch.empty(n, dtype=torch.float32, device=qkv.device)
+      status = torch.zeros(1, dtype=torch.int32, device=qkv.device)
+    code = _entry("mi_attention_tree_tc", "ppppi" + "ppppp" + "ippppi" + "iiiiiiiiiffp")(
+      *head, *where, scratch.data_ptr(), status.data_ptr(), *sizes, stream)
+    if code != TREE_NOT_TAKEN:
+      _check(common_lib(), code, kernels=2)
+      if ws is None and int(status[0]) != 0:
+        raise KernelError("tree_attention: a bounded wait on a barrier ran out")
+      return
   # pieces of the keys: enough blocks for the GPU, none shorter than a tile
-  blocks = batch.num_items * num_kv_heads * -(-batch.max_q_len * (num_heads // num_kv_heads) // 32)
+  blocks = batch.num_items * num_kv_heads * -(-max_q * (num_heads // num_kv_heads) // 32)
   pieces = max(1, min(4 * _num_sms(qkv.device) // blocks, -(-batch.max_ctx_len // 64)))
   chunk = -(-batch.max_ctx_len // pieces)
   scratch = None
   if pieces > 1:
     n = T * num_heads * pieces * (head_dim + 2)
-    scratch = (batch.scratch.buffer("attention_tree_partials", (n,), torch.float32) if batch.scratch is not None
-               else torch.empty(n, dtype=torch.float32, device=qkv.device))
-  _check(lib, lib.mi_attention_tree(_ptr(out), _ptr(qkv), dt, _ptr(kv_layer), *where, _ptr(scratch), *sizes, chunk, pieces, _stream()),
-         kernels=1 + int(pieces > 1))
+    scratch = ws.buffer("attention_tree_partials", (n,), torch.float32) if ws is not None else torch.empty(n, dtype=torch.float32, device=qkv.device)
+  code = _entry("mi_attention_tree", "ppippi" + "ppppp" + "ippp" + "iiiiiiiiiiffiip")(
+    *head, dt, *where, scratch.data_ptr() if scratch is not None else 0, *sizes, chunk, pieces, stream)
+  _check(common_lib(), code, kernels=1 + int(pieces > 1))
+
+
+TREE_NOT_TAKEN = 2      # what mi_attention_tree_tc answers for sizes or addresses that it leaves to mi_attention_tree
+_tree_floats: Dict[tuple, int] = {}
+
+
+def _tree_tc_floats(num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_q: int) -> int:
+  """Floats of scratch that the tcgen05 kernel wants for these sizes; 0: it does not take them."""
+  key = (num_heads, num_kv_heads, head_dim, page_size, max_q)
+  n = _tree_floats.get(key)
+  if n is None:
+    if len(_tree_floats) > 4096:
+      _tree_floats.clear()
+    n = _tree_floats[key] = int(_entry("mi_attention_tree_tc_floats", "iiiii", "l")(*key))
+  return n
 
 
 class _AttentionOptions:
