@@ -3,7 +3,7 @@
 // sees.
 //
 // A block has BR query rows of one (item, key/value head) and a piece of the item's keys, walked in tiles of BK: an online softmax in base 2,
-// scores and weighted values by FMAs from shared memory, 4 rows and BK / TX keys (then values) a thread, so a value read from shared
+// scores and weighted values by FMAs from shared memory, four rows a warp and BK / 32 keys (then values) a lane, so a value read from shared
 // memory serves four products.  The rows of a head group lie side by side: a key is fetched once for all of them.  Pieces give a small
 // step enough blocks; more than one of them leave sums that tree_merge_kernel puts together.
 //
@@ -16,7 +16,8 @@ namespace {
 
 using namespace mi_tree;
 
-constexpr int THREADS = 128;
+// A warp has four rows.
+constexpr int threads_of(int rows) { return rows * 8; }
 
 template <typename T>
 __device__ __forceinline__ void load_row4(float4& v, const T* p, int left, bool wide) {      // four values, zeros past the row
@@ -34,14 +35,16 @@ __device__ __forceinline__ void load_row4(float4& v, const T* p, int left, bool 
 
 // grid: (pieces, row tiles * nkv, items)
 template <typename T, int BR, int BK, int HD>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(threads_of(BR))
 tree_kernel(Args a, int chunk, int pieces, int wide) {
-  constexpr int TX = THREADS / (BR / 4), KEYS = BK / TX, COLS = HD / (4 * TX);
-  static_assert(BK % TX == 0 && HD % (4 * TX) == 0 && TX <= 32, "a row's threads share a warp");
+  constexpr int THREADS = threads_of(BR), TX = 32, KEYS = BK / TX, COLS = HD / (4 * TX);
+  static_assert(BK % TX == 0 && HD % (4 * TX) == 0, "a row's threads are a warp's");
   extern __shared__ __align__(16) float smem[];
   const int hd4 = (a.hd + 3) / 4, stride = 4 * hd4 + 4;      // a row in shared memory, 16 bytes on for the banks
-  float *q_s = smem, *k_s = q_s + BR * stride, *p_s = k_s + BK * stride;      // [BR, stride], [BK, stride] (keys, then values), [BR, BK + 4]
+  float *q_s = smem, *k_s = q_s + BR * stride, *v_s = k_s + BK * stride, *p_s = v_s + BK * stride;      // [BR, stride], [BK, stride] twice, [BR, BK + 4]
   constexpr int PS = BK + 4;
+  __shared__ const T* rows_of[2][BK];      // of this tile's keys and of the next one's: where in the cache the key lies; the values so much further on
+  const size_t to_values = (size_t)a.nkv * a.page_size * a.hd;
   const int piece = blockIdx.x, head = blockIdx.y % a.nkv, r0 = blockIdx.y / a.nkv * BR;
   mi::grid_dependency_sync();
   const Item it = item_of(a, blockIdx.z);
@@ -76,20 +79,39 @@ tree_kernel(Args a, int chunk, int pieces, int wide) {
 #pragma unroll
     for (int c = 0; c < COLS; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
   }
-  auto load_tile = [&](int key0, int which) {
-    for (int i = threadIdx.x; i < BK * hd4; i += THREADS) {
-      const int k = i / hd4, d = 4 * (i - k * hd4), key = key0 + k;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (key < key_end) {
-        const size_t row = (((size_t)page_of(a, it, key) * 2 + which) * a.nkv + head) * a.page_size + key % a.page_size;
-        load_row4(v, kv + row * a.hd + d, a.hd - d, wide);
-      }
-      *reinterpret_cast<float4*>(k_s + k * stride + d) = v;
+  auto find_rows = [&](int key0, int buffer) {
+    for (int k = threadIdx.x; k < BK; k += THREADS) {
+      const int key = key0 + k;
+      rows_of[buffer][k] = key < key_end ? kv + (((size_t)page_of(a, it, key) * 2 * a.nkv + head) * a.page_size + key % a.page_size) * a.hd : nullptr;
     }
   };
-  for (int key0 = key_begin; key0 < key_end; key0 += BK) {
-    __syncthreads();
-    load_tile(key0, 0);
+  // A tile's keys or values on their way (float32 by asynchronous copies, where a row is whole 16 bytes); zeros past the piece.
+  auto load_tile = [&](float* to, int buffer, size_t further) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < BK * hd4; i += THREADS) {
+      const int k = i / hd4, d = 4 * (i - k * hd4);
+      const T* from = rows_of[buffer][k];
+      float* dst = to + k * stride + d;
+      if (sizeof(T) == 4 && wide) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(from ? from + further + d : kv), "r"(from ? 16 : 0) : "memory");
+      } else {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (from) load_row4(v, from + further + d, a.hd - d, wide);
+        *reinterpret_cast<float4*>(dst) = v;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // the keys of a tile are on their way while the values of the tile before are worked on, its values while its scores are made
+  find_rows(key_begin, 0);
+  __syncthreads();
+  load_tile(k_s, 0, 0);
+  load_tile(v_s, 0, to_values);
+  int buffer = 0;
+  for (int key0 = key_begin; key0 < key_end; key0 += BK, buffer ^= 1) {
+    const bool more = key0 + BK < key_end;
+    if (more) find_rows(key0 + BK, buffer ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");      // the keys are there
     __syncthreads();
     float s[4][KEYS];
 #pragma unroll
@@ -142,29 +164,43 @@ tree_kernel(Args a, int chunk, int pieces, int wide) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][c][e] *= alpha;
     }
-    __syncthreads();
-    load_tile(key0, 1);
+    __syncthreads();      // (scores made, weights written)
+    if (more) {
+      load_tile(k_s, buffer ^ 1, 0);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");      // the values are there
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
     __syncthreads();
     const bool all = key0 + BK <= min(it.start, key_end) && a.window <= 0;      // every row sees every key of the tile
     const int near = min(BK, key_end - key0);
-    for (int k = 0; k < near; ++k) {
-      float p[4];
+    for (int k0 = 0; k0 < near; k0 += 4) {      // (past `near` all weights are -1)
+      float4 p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = p_s[(4 * ty + i) * PS + k];
+      for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(p_s + (4 * ty + i) * PS + k0);
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) {
-        const int d = 4 * (tx + TX * c);
-        if (d >= 4 * hd4) break;
-        const float4 v = *reinterpret_cast<const float4*>(k_s + k * stride + d);
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (all || !(p[i] < 0.f)) {
-            acc[i][c][0] = fmaf(p[i], v.x, acc[i][c][0]);
-            acc[i][c][1] = fmaf(p[i], v.y, acc[i][c][1]);
-            acc[i][c][2] = fmaf(p[i], v.z, acc[i][c][2]);
-            acc[i][c][3] = fmaf(p[i], v.w, acc[i][c][3]);
+        for (int c = 0; c < COLS; ++c) {
+          const int d = 4 * (tx + TX * c);
+          if (d < 4 * hd4) {
+            const float4 v = *reinterpret_cast<const float4*>(v_s + (k0 + k) * stride + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float w = k == 0 ? p[i].x : k == 1 ? p[i].y : k == 2 ? p[i].z : p[i].w;
+              if (all || !(w < 0.f)) {
+                acc[i][c][0] = fmaf(w, v.x, acc[i][c][0]);
+                acc[i][c][1] = fmaf(w, v.y, acc[i][c][1]);
+                acc[i][c][2] = fmaf(w, v.z, acc[i][c][2]);
+                acc[i][c][3] = fmaf(w, v.w, acc[i][c][3]);
+              }
+            }
           }
-      }
+        }
+    }
+    if (more) {
+      __syncthreads();
+      load_tile(v_s, buffer ^ 1, to_values);
     }
   }
 #pragma unroll
@@ -213,38 +249,57 @@ tree_merge_kernel(Args a, int chunk, int pieces) {
   const int n = min((ctx + chunk - 1) / chunk, pieces);
   const size_t at = (size_t)t * a.nh + h;
   const float sink2 = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
-  float top = sink2;
-  for (int s = lane; s < n; s += 32) top = fmaxf(top, a.part_ml[2 * (at * pieces + s)]);
-  top = mi::warp_max(top);
-  const float off = top == -INFINITY ? 0.f : top;
-  float total = exp2f(sink2 - off);
-  for (int s = 0; s < n; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at * pieces + s));
-    total = fmaf(ml.y, exp2f(ml.x - off), total);
-  }
-  for (int d = lane; d < a.hd; d += 32) {
-    float sum = 0.f;
-    for (int s = 0; s < n; ++s) sum = fmaf(a.part_o[(at * pieces + s) * a.hd + d], exp2f(a.part_ml[2 * (at * pieces + s)] - off), sum);
-    reinterpret_cast<T*>(a.out)[at * a.hd + d] = mi::from_float<T>(total == 0.f ? 0.f : sum / total);
+  constexpr int AT_ONCE = 8, COLS = 4;      // pieces and 32s of columns that are on their way at a time
+  for (int d0 = lane; d0 < a.hd; d0 += 32 * COLS) {
+    float top = sink2, total = a.sink ? 1.f : 0.f, sum[COLS] = {};
+    for (int s0 = 0; s0 < n; s0 += AT_ONCE) {
+      float2 ml[AT_ONCE];
+      float x[AT_ONCE][COLS];
+#pragma unroll
+      for (int s = 0; s < AT_ONCE; ++s) {
+        const bool there = s0 + s < n;
+        ml[s] = there ? *reinterpret_cast<const float2*>(a.part_ml + 2 * (at * pieces + s0 + s)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) x[s][c] = there && d0 + 32 * c < a.hd ? a.part_o[(at * pieces + s0 + s) * a.hd + d0 + 32 * c] : 0.f;
+      }
+      float next = top;
+#pragma unroll
+      for (int s = 0; s < AT_ONCE; ++s) next = fmaxf(next, ml[s].x);
+      const float off = next == -INFINITY ? 0.f : next, alpha = exp2f(top - off);
+      top = next;
+      total *= alpha;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) sum[c] *= alpha;
+#pragma unroll
+      for (int s = 0; s < AT_ONCE; ++s) {
+        const float w = exp2f(ml[s].x - off);
+        total = fmaf(ml[s].y, w, total);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) sum[c] = fmaf(x[s][c], w, sum[c]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < COLS; ++c)
+      if (d0 + 32 * c < a.hd) reinterpret_cast<T*>(a.out)[at * a.hd + d0 + 32 * c] = mi::from_float<T>(total == 0.f ? 0.f : sum[c] / total);
   }
 }
 
 template <typename T, int BR, int BK, int HD>
 int launch(const Args& a, int chunk, int pieces, bool wide, cudaStream_t stream) {
   const int stride = (a.hd + 3) / 4 * 4 + 4;
-  const size_t smem = ((size_t)(BR + BK) * stride + BR * (BK + 4)) * sizeof(float);
+  const size_t smem = ((size_t)(BR + 2 * BK) * stride + BR * (BK + 4)) * sizeof(float);
   static bool ready[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return mi_fail("attention_tree: no current device");
   if (!ready[dev]) {
-    const size_t most = ((size_t)(BR + BK) * (HD + 4) + BR * (BK + 4)) * sizeof(float);
+    const size_t most = ((size_t)(BR + 2 * BK) * (HD + 4) + BR * (BK + 4)) * sizeof(float);
     if (cudaFuncSetAttribute(tree_kernel<T, BR, BK, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
       return mi_fail("attention_tree: %zu bytes of shared memory were refused", most);
     ready[dev] = true;
   }
   const int tiles = (a.max_q * a.G + BR - 1) / BR;
   MI_REQUIRE((long long)tiles * a.nkv <= 65535, "attention_tree: %d rows of %d heads are too many for one launch", a.max_q * a.G, a.nkv);
-  if (mi::launch(tree_kernel<T, BR, BK, HD>, dim3(pieces, tiles * a.nkv, a.items), dim3(THREADS), smem, stream, a, chunk, pieces, (int)wide) != cudaSuccess)
+  if (mi::launch(tree_kernel<T, BR, BK, HD>, dim3(pieces, tiles * a.nkv, a.items), dim3(threads_of(BR)), smem, stream, a, chunk, pieces, (int)wide) != cudaSuccess)
     return mi_fail("attention_tree: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   if (pieces > 1 && mi::launch(tree_merge_kernel<T>, dim3(a.T, (a.nh + 3) / 4), dim3(128), 0, stream, a, chunk, pieces) != cudaSuccess)
     return mi_fail("attention_tree: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
@@ -269,7 +324,11 @@ MI_API int mi_attention_tree(void* out, const void* qkv, int dtype, const void* 
          scratch + (size_t)T * nh * pieces * 2, scratch, items, T, width, nh, nkv, nh / nkv, hd, pages, page_size, window, max_q, scale, softcap};
   const int size = dtype == MI_F32 ? 4 : 2;
   const bool wide = hd % 4 == 0 && (long long)width % 4 == 0 && (((uintptr_t)qkv | (uintptr_t)kv) % (4 * size)) == 0;
-  if (dtype == MI_F32) return hd <= 256 ? launch<float, 32, 64, 256>(a, chunk, pieces, wide, stream) : launch<float, 16, 32, 640>(a, chunk, pieces, wide, stream);
-  MI_REQUIRE(dtype == MI_BF16, "attention_tree: unknown type");
+  MI_REQUIRE(dtype == MI_F32 || dtype == MI_BF16, "attention_tree: unknown type");
+  if (dtype == MI_F32) {
+    if (hd <= 128) return launch<float, 32, 64, 128>(a, chunk, pieces, wide, stream);
+    return hd <= 256 ? launch<float, 32, 64, 256>(a, chunk, pieces, wide, stream) : launch<float, 16, 32, 640>(a, chunk, pieces, wide, stream);
+  }
+  if (hd <= 128) return launch<__nv_bfloat16, 32, 64, 128>(a, chunk, pieces, wide, stream);
   return hd <= 256 ? launch<__nv_bfloat16, 32, 64, 256>(a, chunk, pieces, wide, stream) : launch<__nv_bfloat16, 16, 32, 640>(a, chunk, pieces, wide, stream);
 }

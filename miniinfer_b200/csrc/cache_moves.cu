@@ -17,7 +17,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int MAX_PAIRS = 4096;                // of one call of `places`: a column of 16 bytes of each fits a block's shared memory
-constexpr int SMEM_WANTED = 48 << 10;          // four blocks of this size share an SM and take turns at reading and writing
+constexpr int SMEM_WANTED = 32 << 10;          // six blocks of this size share an SM and take turns at reading and writing (0.12 GB of rows: 20.5 us; by 48 KB 22.9)
 constexpr int SMEM_MOST = 200 << 10;
 
 template <typename U>
@@ -39,31 +39,36 @@ struct Places {
   void* base;
   const int *src, *dst, *filled;      // [n]; filled or null: the first filled[k] of a place's `page` rows only
   long long places, row_units;        // places of a layer; units of a place
-  int n, columns;                     // pairs; columns (units) of a block
+  int n, log_columns;                 // pairs; columns (units) of a block, a power of two
   int page, token_units;              // rows of a head's part of a place, units of such a row
 };
 
-// One block: columns blockIdx.x * columns .. of layer blockIdx.y, of all pairs.
+// One block: a few columns of layer blockIdx.y, of all pairs.  A thread stays in its column; 2^log_columns threads side by side take a pair.
 template <typename U, bool FILLED>
 __global__ void __launch_bounds__(THREADS) move_places_kernel(Places a) {
   extern __shared__ __align__(16) unsigned char smem[];
   U* stage = reinterpret_cast<U*>(smem);                                                     // [n, columns]
-  const long long c0 = (long long)blockIdx.x * a.columns;
-  const int cols = (int)min((long long)a.columns, a.row_units - c0), total = a.n * cols;
-  U* layer = reinterpret_cast<U*>(a.base) + (long long)blockIdx.y * a.places * a.row_units + c0;
+  const int columns = 1 << a.log_columns, c = threadIdx.x & (columns - 1), k0 = threadIdx.x >> a.log_columns, step = THREADS >> a.log_columns;
+  const long long at = ((long long)blockIdx.x << a.log_columns) + c;
+  U* column = reinterpret_cast<U*>(a.base) + (long long)blockIdx.y * a.places * a.row_units + at;
+  const int row = FILLED ? (int)(at / a.token_units % a.page) : 0;
   mi::grid_dependency_sync();
-  auto wanted = [&](int k, int c, int from, int to) {
-    if ((unsigned)from >= (unsigned long long)a.places || (unsigned)to >= (unsigned long long)a.places || from == to) return false;
-    return !FILLED || (int)((c0 + c) / a.token_units % a.page) < a.filled[k];
-  };
-  for (int i = threadIdx.x; i < total; i += THREADS) {
-    const int k = i / cols, c = i - k * cols, from = a.src[k];
-    if (wanted(k, c, from, a.dst[k])) copy_to_shared(stage + i, layer + from * a.row_units + c);
+  if (at < a.row_units) {
+#pragma unroll 4
+    for (int k = k0; k < a.n; k += step) {
+      const int from = a.src[k], to = a.dst[k];
+      const bool wanted = (unsigned)from < (unsigned long long)a.places && (unsigned)to < (unsigned long long)a.places && from != to && (!FILLED || row < a.filled[k]);
+      if (wanted) copy_to_shared(stage + (k << a.log_columns) + c, column + from * a.row_units);
+    }
   }
   copies_done();
-  for (int i = threadIdx.x; i < total; i += THREADS) {
-    const int k = i / cols, c = i - k * cols, to = a.dst[k];
-    if (wanted(k, c, a.src[k], to)) layer[to * a.row_units + c] = stage[i];
+  if (at < a.row_units) {
+#pragma unroll 4
+    for (int k = k0; k < a.n; k += step) {
+      const int from = a.src[k], to = a.dst[k];
+      const bool wanted = (unsigned)from < (unsigned long long)a.places && (unsigned)to < (unsigned long long)a.places && from != to && (!FILLED || row < a.filled[k]);
+      if (wanted) column[to * a.row_units] = stage[(k << a.log_columns) + c];
+    }
   }
 }
 
@@ -73,34 +78,53 @@ struct Rows {
   long long pages;
   int pairs, planes, plane_step;      // pairs in all; (layer, key or value, head) triples, and how many of them a block takes
   int heads2, page, row_units, most;  // key and value heads of a layer; units of a row; rows of a group that are moved at a time
+  int columns, log_lanes;             // units of a row that are moved at a time, all of them where they fit; 2^log_lanes threads side by side take them
 };
 
-// One block: plane_step planes of group blockIdx.y, `most` rows at a time.
+// One block: plane_step planes of group blockIdx.y, `most` rows at a time.  An address is the sum of two numbers, of the pair and of the plane: tables, for
+// divisions would cost more than the copies.
 template <typename U>
 __global__ void __launch_bounds__(THREADS) move_rows_kernel(Rows a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  U* stage = reinterpret_cast<U*>(smem);                                                     // [planes of the block, most, row_units]
+  longlong2* of_pair = reinterpret_cast<longlong2*>(smem);                                   // [most]: from, to; -1: nothing to do
+  long long* of_plane = reinterpret_cast<long long*>(of_pair + a.most);                      // [plane_step]
+  U* stage = reinterpret_cast<U*>(smem + (a.most * 16 + a.plane_step * 8 + 15) / 16 * 16);   // [planes of the block, rows, columns]
   const int p0 = blockIdx.x * a.plane_step, planes = min(a.plane_step, a.planes - p0);
+  const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), first = threadIdx.x >> a.log_lanes, step = THREADS >> a.log_lanes;
+  for (int p = threadIdx.x; p < planes; p += THREADS)
+    of_plane[p] = ((long long)((p0 + p) / a.heads2) * a.pages * a.heads2 + (p0 + p) % a.heads2) * a.page * a.row_units;
   mi::grid_dependency_sync();
   const int lo = max(a.start[blockIdx.y], 0), hi = min(a.start[blockIdx.y + 1], a.pairs);
   const long long limit = a.pages * a.page;
-  auto at = [&](int plane, int place) {      // of (layer, w * heads + h)
-    const long long page = (long long)(plane / a.heads2) * a.pages + place / a.page;
-    return ((page * a.heads2 + plane % a.heads2) * a.page + place % a.page) * a.row_units;
-  };
   U* base = reinterpret_cast<U*>(a.base);
+  auto of_place = [&](int place) { return ((long long)(place / a.page) * a.heads2 * a.page + place % a.page) * a.row_units; };
   for (int k0 = lo; k0 < hi; k0 += a.most) {
-    const int rows = min(a.most, hi - k0), width = rows * a.row_units, total = planes * width;
-    for (int i = threadIdx.x; i < total; i += THREADS) {
-      const int p = i / width, k = k0 + (i - p * width) / a.row_units, u = i % a.row_units, from = a.src[k], to = a.dst[k];
-      if ((unsigned)from < limit && (unsigned)to < limit && from != to) copy_to_shared(stage + i, base + at(p0 + p, from) + u);
-    }
-    copies_done();
-    for (int i = threadIdx.x; i < total; i += THREADS) {
-      const int p = i / width, k = k0 + (i - p * width) / a.row_units, u = i % a.row_units, from = a.src[k], to = a.dst[k];
-      if ((unsigned)from < limit && (unsigned)to < limit && from != to) base[at(p0 + p, to) + u] = stage[i];
+    const int rows = min(a.most, hi - k0), total = planes * rows;
+    for (int k = threadIdx.x; k < rows; k += THREADS) {
+      const int from = a.src[k0 + k], to = a.dst[k0 + k];
+      const bool wanted = (unsigned)from < limit && (unsigned)to < limit && from != to;
+      of_pair[k] = wanted ? make_longlong2(of_place(from), of_place(to)) : make_longlong2(-1, -1);
     }
     __syncthreads();
+    for (int c0 = 0; c0 < a.row_units; c0 += a.columns) {
+      const int columns = min(a.columns, a.row_units - c0);
+#pragma unroll 4
+      for (int i = first; i < total; i += step) {
+        const int p = i / rows;
+        const long long from = of_pair[i - p * rows].x;
+        if (from >= 0)
+          for (int u = lane; u < columns; u += 1 << a.log_lanes) copy_to_shared(stage + i * a.columns + u, base + of_plane[p] + from + c0 + u);
+      }
+      copies_done();
+#pragma unroll 4
+      for (int i = first; i < total; i += step) {
+        const int p = i / rows;
+        const long long to = of_pair[i - p * rows].y;
+        if (to >= 0)
+          for (int u = lane; u < columns; u += 1 << a.log_lanes) base[of_plane[p] + to + c0 + u] = stage[i * a.columns + u];
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -126,17 +150,16 @@ template <typename U, bool FILLED>
 int launch_places(Places a, int layers, cudaStream_t stream) {
   static bool ready[64] = {};
   if (allow_shared(move_places_kernel<U, FILLED>, ready)) return 1;
-  // columns: what the wanted shared memory holds, at least 8 (128 bytes in a row) as long as the most allows, and few enough that small
-  // calls are spread over the GPU
+  // columns: what the wanted shared memory holds, at least 8 (128 bytes in a row) as long as the most allows, no more than a place or the threads have,
+  // and few enough that small calls are spread over the GPU
   const long long per = (long long)a.n * sizeof(U), spread = (a.row_units * layers + 4 * mi::sm_count() - 1) / (4 * mi::sm_count());
-  long long c = SMEM_WANTED / per;
-  if (c < 8) c = 8;
-  if (c > SMEM_MOST / per) c = SMEM_MOST / per;
-  const long long least = spread > 16 ? spread : 16;
-  if (c > least) c = least;
-  if (c > a.row_units) c = a.row_units;
-  a.columns = (int)c;
-  const long long blocks = (a.row_units + c - 1) / c;
+  long long most = SMEM_WANTED / per;
+  if (most < 8) most = 8;
+  if (most > SMEM_MOST / per) most = SMEM_MOST / per;
+  if (most > (spread > 16 ? spread : 16)) most = spread > 16 ? spread : 16;
+  a.log_columns = 0;
+  while ((2ll << a.log_columns) <= most && (2 << a.log_columns) <= THREADS && (1ll << a.log_columns) < a.row_units) ++a.log_columns;
+  const long long c = 1ll << a.log_columns, blocks = (a.row_units + c - 1) / c;
   MI_REQUIRE(blocks <= 0x7fffffffll && layers <= 65535, "cache moves: %lld blocks of %d layers are too many for one launch", blocks, layers);
   if (mi::launch(move_places_kernel<U, FILLED>, dim3((unsigned)blocks, layers), dim3(THREADS), (size_t)(per * c), stream, a) != cudaSuccess)
     return mi_fail("cache moves: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
@@ -148,15 +171,18 @@ template <typename U>
 int launch_rows(Rows a, int groups, cudaStream_t stream) {
   static bool ready[64] = {};
   if (allow_shared(move_rows_kernel<U>, ready)) return 1;
-  const long long row = (long long)a.row_units * sizeof(U);
-  MI_REQUIRE(row <= SMEM_MOST, "move_cache_rows: rows of %lld bytes are too long", row);
-  if (a.most > SMEM_MOST / row) a.most = (int)(SMEM_MOST / row);
-  const long long per = row * a.most, spread = ((long long)a.planes * groups + 4 * mi::sm_count() - 1) / (4 * mi::sm_count());
+  // columns: whole rows, or where `most` of them do not fit as much of each as does: units are moved one by one, so what is read before what stays so
+  const long long units = (SMEM_MOST - 64 - 16ll * a.most) / (a.most * (long long)sizeof(U));
+  MI_REQUIRE(units >= 1, "move_cache_rows: most=%d rows at a time are too many", a.most);
+  a.columns = units < a.row_units ? (int)units : a.row_units;
+  const long long per = (long long)a.columns * sizeof(U) * a.most + 8, spread = ((long long)a.planes * groups + 4 * mi::sm_count() - 1) / (4 * mi::sm_count());
   long long step = SMEM_WANTED / per;
   if (step > spread) step = spread;
   if (step < 1) step = 1;
   a.plane_step = (int)step;
-  if (mi::launch(move_rows_kernel<U>, dim3((unsigned)((a.planes + step - 1) / step), groups), dim3(THREADS), (size_t)(per * step), stream, a) != cudaSuccess)
+  a.log_lanes = 0;
+  while ((1 << a.log_lanes) < a.columns && (2 << a.log_lanes) <= THREADS) ++a.log_lanes;
+  if (mi::launch(move_rows_kernel<U>, dim3((unsigned)((a.planes + step - 1) / step), groups), dim3(THREADS), (size_t)(per * step + a.most * 16 + 16), stream, a) != cudaSuccess)
     return mi_fail("move_cache_rows: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   MI_LAUNCH_OK("move_cache_rows");
   return 0;
@@ -195,7 +221,7 @@ MI_API int mi_move_cache_rows(void* base, int layers, long long pages, int heads
   MI_REQUIRE(pages * page <= 0x7fffffffll && 2ll * layers * heads <= 0x7fffffffll && groups <= 65535, "move_cache_rows: %lld pages of %d rows or %d groups are too many", pages, page, groups);
   const int unit = unit_of(base, row_bytes);
   if (most > pairs) most = pairs;
-  Rows a{base, src, dst, start, pages, pairs, 2 * layers * heads, 0, 2 * heads, page, (int)(row_bytes / unit), most};
+  Rows a{base, src, dst, start, pages, pairs, 2 * layers * heads, 0, 2 * heads, page, (int)(row_bytes / unit), most, 0, 0};
   if (unit == 16) return launch_rows<uint4>(a, groups, stream);
   if (unit == 4) return launch_rows<uint32_t>(a, groups, stream);
   if (unit == 2) return launch_rows<uint16_t>(a, groups, stream);

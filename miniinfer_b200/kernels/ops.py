@@ -1700,16 +1700,17 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
       if ws is None and int(status[0]) != 0:
         raise KernelError("tree_attention: a bounded wait on a barrier ran out")
       return
-  # pieces of the keys: enough blocks for the GPU, none shorter than a tile
+  # pieces of the keys, of whole tiles of 64: up to four blocks an SM, two of which it holds at a time (heads of 128; requests differ in length)
   blocks = batch.num_items * num_kv_heads * -(-max_q * (num_heads // num_kv_heads) // 32)
   pieces = max(1, min(4 * _num_sms(qkv.device) // blocks, -(-batch.max_ctx_len // 64)))
-  chunk = -(-batch.max_ctx_len // pieces)
+  chunk = -(-batch.max_ctx_len // (64 * pieces)) * 64
+  pieces = max(1, -(-batch.max_ctx_len // chunk)) if chunk else 1
   scratch = None
   if pieces > 1:
     n = T * num_heads * pieces * (head_dim + 2)
     scratch = ws.buffer("attention_tree_partials", (n,), torch.float32) if ws is not None else torch.empty(n, dtype=torch.float32, device=qkv.device)
   code = _entry("mi_attention_tree", "ppippi" + "ppppp" + "ippp" + "iiiiiiiiiiffiip")(
-    *head, dt, *where, scratch.data_ptr() if scratch is not None else 0, *sizes, chunk, pieces, stream)
+    *head, dt, *where, scratch.data_ptr() if scratch is not None else 0, *sizes, max(chunk, 1), pieces, stream)
   _check(common_lib(), code, kernels=1 + int(pieces > 1))
 
 

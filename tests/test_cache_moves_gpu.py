@@ -100,6 +100,14 @@ def test_move_cache_rows(layers, groups, nodes, kept, heads, P, hd, dtype):
       compare("move_cache_rows", kv, ints(src), ints(dst), ints(start), most)
 
 
+def test_rows_that_change_places_and_do_not_fit_a_block_whole():
+  """A cycle through more bytes of rows than a block's shared memory holds: still read before they are written."""
+  for dtype, dim in ((torch.float32, 512), (torch.bfloat16, 36)):
+    kv = filled_tensor((1, 20, 2, 1, 64, dim), dtype, dim)
+    places = random.Random(1).sample(range(64, 20 * 64), 1100)
+    compare("move_cache_rows", kv, ints(places), ints(places[1:] + places[:1]), ints([0, 1100]), 1100)
+
+
 def test_places_that_pass_32_bits():
   """Offsets in bytes and in values beyond 2^32: 5 GiB of pages, the last of them."""
   if DEV == "cpu":
