@@ -9,7 +9,9 @@ Against the reference (miniinfer/kvcache/kv_cache_manager.py, memory_pool.py):
   * page 0 of every pool is a dummy that padded tokens may write to (memory_pool.py:422-424);
   * a request keeps its slot and pages from admission to release, also between portions of its
     prompt (the reference frees the slot between chunks, llm_engine.py:1178-1181);
-  * pages behind a layer group's window or chunk are given back as soon as no later query can see them.
+  * pages behind a layer group's window or chunk are given back as soon as no later query can see them;
+  * a request may be forked: the copies share its full pages, which are counted and go back when the last request lets go of them (the
+    reference shares pages through its radix tree only, miniinfer/kvcache/radix_cache.py), and have a last, partly filled page of their own.
 
 The manager does no scheduling: callers ask ``can_append`` and then ``append``; ``commit`` makes
 the appended tokens part of the request after the step has run.
@@ -18,13 +20,15 @@ the appended tokens part of the request after the step has run.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, Hashable, List, Optional, Sequence
+from collections import Counter
+from typing import Dict, Hashable, List, Mapping, Optional, Sequence
 
 import numpy as np
 import torch
 
 STAGING_SLOTS = 8     # pinned snapshots of a block table that uploads in flight may still read
 
+from ..kernels import ops
 from .specs import CacheSpec, CompositeSpec, FixedStateSpec, PagedKVSpec, flatten_specs
 
 
@@ -38,14 +42,15 @@ class OutOfSlots(RuntimeError):
 
 class PageAllocator:
   """Host free list of the page ids ``1..num_pages`` (0 is the dummy page).  Last freed, first
-  reused.  Holding a page twice or freeing it twice is an error."""
+  reused.  A page has one holder when it is handed out and one more for each ``share``; it is free when the last has freed it.  Freeing a
+  page that nobody holds is an error."""
 
   def __init__(self, num_pages: int):
     if num_pages < 1:
       raise ValueError("a pool needs at least one page")
     self.num_pages = num_pages
     self._free: List[int] = list(range(num_pages, 0, -1))
-    self._held = bytearray(num_pages + 1)
+    self._held = [0] * (num_pages + 1)      # holders of each page
 
   @property
   def num_free(self) -> int:
@@ -61,12 +66,23 @@ class PageAllocator:
       self._held[p] = 1
     return out
 
+  def share(self, pages: Sequence[int]) -> None:
+    """One holder more for each of the pages."""
+    for p in pages:
+      if p <= 0 or p > self.num_pages or not self._held[p]:
+        raise AssertionError(f"page {p} shared but not held")
+      self._held[p] += 1
+
   def free(self, pages: Sequence[int]) -> None:
     for p in pages:
       if p <= 0 or p > self.num_pages or not self._held[p]:
         raise AssertionError(f"page {p} freed but not held")
-      self._held[p] = 0
-      self._free.append(p)
+      self._held[p] -= 1
+      if not self._held[p]:
+        self._free.append(p)
+
+  def holders(self, page: int) -> int:
+    return self._held[page]
 
   def held(self) -> List[int]:
     return [p for p in range(1, self.num_pages + 1) if self._held[p]]
@@ -377,6 +393,10 @@ class KVCacheManager:
   def release_request(self, req_id: Hashable) -> None:
     """Gives back everything the request holds (miniinfer/kvcache/kv_cache_manager.py:664)."""
     r = self._requests.pop(req_id)
+    self._give_back(r)
+    self._free_slots.append(r.slot)
+
+  def _give_back(self, r: _Request) -> None:
     for g in self.paged_groups:
       live = [p for p in r.pages[g.index] if p != 0]
       if live:
@@ -385,7 +405,122 @@ class KVCacheManager:
       if n:
         g.block_table_host[r.slot, :n] = 0
         g._dirty.add(r.slot)
-    self._free_slots.append(r.slot)
+
+  # ------------------------------------------------------------------ several continuations of a request
+
+  def _settled(self, req_id: Hashable) -> _Request:
+    r = self._requests[req_id]
+    if r.reserved:
+      raise ValueError(f"request {req_id!r} has {r.reserved} tokens that are neither committed nor cancelled")
+    return r
+
+  def _copy_of(self, r: _Request, slot: int, copies: List[List[tuple]]) -> _Request:
+    """A request in ``slot`` that goes on from where ``r`` is: its full pages shared, a page of its own for what a last page holds.  The pages to
+    copy - (from, to, tokens) - are put into ``copies``, a list a group; the caller has seen to it that there are pages."""
+    new = _Request(slot=slot, length=r.length, pages=[list(p) for p in r.pages])
+    for g, todo in zip(self.paged_groups, copies):
+      mine, filled = new.pages[g.index], r.length % g.page_size
+      if filled:
+        page = g.allocator.alloc(1)[0]
+        todo.append((mine[-1], page, filled))
+        mine[-1] = page
+      g.allocator.share([p for p in (mine[:-1] if filled else mine) if p])
+      g.block_table_host[slot, :len(mine)] = mine
+      g._dirty.add(slot)
+    return new
+
+  def _copy_on_device(self, copies: List[List[tuple]], slots: List[tuple]) -> None:
+    """The pages' copies, a launch a group, and those of the states of ``slots`` - (from, to)."""
+    def lists(rows):
+      return torch.tensor(rows, dtype=torch.int32).t().contiguous().to(self.device)
+
+    for g, todo in zip(self.paged_groups, copies):
+      for i in range(0, len(todo), ops.MOVE_MAX_PAIRS):
+        src, dst, filled = lists(todo[i:i + ops.MOVE_MAX_PAIRS])
+        ops.copy_cache_pages(g.kv, src, dst, filled)
+    if slots:
+      src, dst = lists(slots)
+      for s in self.state_groups:
+        ops.reorder_states(s.state, src, dst)
+
+  def fork(self, req_id: Hashable, children: Sequence[Hashable]) -> None:
+    """Admits ``children``, each of which goes on from where the request is, its states with it: full pages are shared, what the last, partly
+    filled page holds is copied.  ``OutOfSlots`` or ``OutOfPages`` change nothing."""
+    r, n = self._settled(req_id), len(children)
+    if len(set(children)) < n or any(c in self._requests for c in children):
+      raise KeyError("a child is already admitted, or named twice")
+    if n > len(self._free_slots):
+      raise OutOfSlots(f"{n} request slots wanted, {len(self._free_slots)} free")
+    for g in self.paged_groups:
+      if r.length % g.page_size and n > g.allocator.num_free:
+        raise OutOfPages(f"group {g.index}: {n} pages wanted for copies of request {req_id!r}, {g.allocator.num_free} of {g.num_pages} free")
+    copies: List[List[tuple]] = [[] for _ in self.paged_groups]
+    slots = []
+    for c in children:
+      slot = self._free_slots.pop()
+      self._requests[c] = self._copy_of(r, slot, copies)
+      slots.append((r.slot, slot))
+    self._copy_on_device(copies, slots)
+
+  def reorder(self, parents: Mapping[Hashable, Hashable]) -> None:
+    """Every request of ``parents`` goes on from where ``parents[request]`` is, all at once: what a beam search's selection asks for.  The
+    parents are requests of the mapping themselves.  A parent's pages and states pass on to one child as they lie; further children get copies
+    as by ``fork``, in the places of the requests that nobody goes on from, whose pages go back.  ``OutOfPages`` changes nothing."""
+    old = {q: self._settled(q) for q in parents}
+    if any(p not in old for p in parents.values()):
+      raise KeyError("a parent is not among the requests that are reordered")
+    heir: Dict[Hashable, Hashable] = {}      # parent -> the child that takes its place over: itself if it goes on
+    for child, parent in parents.items():
+      if parent not in heir or child == parent:
+        heir[parent] = child
+    dropped = [old[q] for q in parents if q not in heir]
+    extra = [(child, parent) for child, parent in parents.items() if heir[parent] != child]
+    for g in self.paged_groups:
+      lost = Counter(p for r in dropped for p in r.pages[g.index] if p)
+      room = g.allocator.num_free + sum(g.allocator.holders(p) == k for p, k in lost.items())
+      # a full page of a dropped request that a copy shares stays held: only pages that no parent holds come back
+      want = sum(1 for _, parent in extra if old[parent].length % g.page_size)
+      if want > room:
+        raise OutOfPages(f"group {g.index}: {want} pages wanted for copies, {room} of {g.num_pages} free")
+    for r in dropped:
+      self._give_back(r)
+    for parent, child in heir.items():
+      self._requests[child] = old[parent]
+    copies: List[List[tuple]] = [[] for _ in self.paged_groups]
+    slots = []
+    for (child, parent), r in zip(extra, dropped):
+      self._requests[child] = self._copy_of(old[parent], r.slot, copies)
+      slots.append((old[parent].slot, r.slot))
+    self._copy_on_device(copies, slots)
+
+  def keep(self, kept: Mapping[Hashable, Sequence[int]]) -> None:
+    """Of the tokens that were appended to each request - the nodes of a drafted tree - those numbered in ``kept`` (rising, from 0) become
+    part of it: their keys and values move to the front, one launch a group for all requests, the tokens are committed, and what the others held
+    goes back.  States cannot be kept in part: with groups of states only a beginning of all tokens can stay, which is all of them."""
+    for req_id, nodes in kept.items():
+      n = self._requests[req_id].reserved
+      if any(not 0 <= a < n for a in nodes) or any(a >= b for a, b in zip(nodes, list(nodes)[1:])):
+        raise ValueError(f"request {req_id!r}: the kept tokens must rise from 0 to below the {n} that were appended")
+      if self.state_groups and len(nodes) != n:
+        raise ValueError(f"request {req_id!r}: a state cannot be kept for {len(nodes)} of {n} tokens")
+    for g in self.paged_groups:
+      src: List[int] = []
+      dst: List[int] = []
+      start = [0]
+      for req_id, nodes in kept.items():
+        first, moved = self._requests[req_id].length, [(a, i) for i, a in enumerate(nodes) if a != i]
+        src += [self.slot_at(req_id, g.index, first + a) for a, _ in moved]
+        dst += [self.slot_at(req_id, g.index, first + i) for _, i in moved]
+        if moved:
+          start.append(len(src))
+      if src:
+        lists = torch.tensor(src + dst + start, dtype=torch.int32).to(self.device)
+        n = len(src)
+        ops.move_cache_rows(g.kv, lists[:n], lists[n:2 * n], lists[2 * n:], max(b - a for a, b in zip(start, start[1:])))
+    for req_id, nodes in kept.items():
+      rest = self._requests[req_id].reserved - len(nodes)
+      self.commit(req_id, len(nodes))
+      self.cancel(req_id, rest)
 
   # ------------------------------------------------------------------ step metadata
 
@@ -429,7 +564,8 @@ class KVCacheManager:
     }
 
   def check_invariants(self) -> None:
-    """No page lost, held twice, or in a block table without an owner."""
+    """No page lost, held by more or fewer requests than are counted, or in a block table without an owner; no page shared that a request
+    may still write."""
     for g in self.paged_groups:
       owned: List[int] = []
       for r in self._requests.values():
@@ -439,9 +575,10 @@ class KVCacheManager:
         n = len(r.pages[g.index])
         assert list(row[:n]) == r.pages[g.index], "block table differs from the request's pages"
         assert not row[n:].any(), "block table has entries past the request's pages"
-      assert len(owned) == len(set(owned)), "a page is held by two requests"
-      assert sorted(owned) == g.allocator.held(), "allocator and requests disagree on held pages"
-      assert len(owned) + g.allocator.num_free == g.num_pages, "a page was lost"
+        assert all(g.allocator.holders(p) == 1 for p in r.pages[g.index][r.length // g.page_size:] if p), "a page that may be written is shared"
+      counts = Counter(owned)
+      assert sorted(counts) == g.allocator.held() and all(g.allocator.holders(p) == k for p, k in counts.items()), "allocator and requests disagree on held pages"
+      assert len(counts) + g.allocator.num_free == g.num_pages, "a page was lost"
     slots = [r.slot for r in self._requests.values()]
     assert len(slots) == len(set(slots)), "a slot is held twice"
     assert sorted(slots + self._free_slots) == list(range(self.max_num_seqs)), "a slot was lost"
