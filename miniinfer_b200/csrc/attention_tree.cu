@@ -50,7 +50,8 @@ tree_kernel(Args a, int chunk, int pieces, int wide) {
   const Item it = item_of(a, blockIdx.z);
   const int rows = it.n * a.G;
   if (r0 >= rows) return;
-  const int key_begin = piece * chunk, key_end = piece == pieces - 1 ? it.ctx : min(it.ctx, key_begin + chunk);
+  const int key_end = piece == pieces - 1 ? it.ctx : min(it.ctx, (piece + 1) * chunk);
+  const int key_begin = max(piece * chunk, window_begin(a, it.start));      // (no new token's position is below the context's length)
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const T* qkv = reinterpret_cast<const T*>(a.qkv);
   const T* kv = reinterpret_cast<const T*>(a.kv);

@@ -41,7 +41,8 @@ struct Tc {
   int boxes, steps, n_out;       // boxes and 16s of columns of a row, columns of P V
   int ring, box_rows;            // units of the ring; rows of a TMA box of keys
   int tokens, max_parts;         // tokens of a set of 128 rows; parts of the largest item
-  float scale_log2;
+  float scale_log2;              // scale * log2(e)
+  float cap_scale, cap_log2;     // with a cap: 2 scale log2(e) / cap, cap log2(e)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -235,24 +236,6 @@ struct Walk {
   }
 };
 
-// 2^x of two values on the multiply-add pipe: x = n + f with f in -1/2 .. 1/2 (adding 1.5 2^23 rounds to the whole number n), a cubic for 2^f
-// fitted to the smallest largest relative error, 1.0e-4, with value 1 at 0 - a twentieth of what rounding to bf16 does -, n added to the
-// exponent.  Below -127: exactly zero, as the cubic is 1 there.  The exponential unit takes 16 values a cycle and SM, and the 256 x 128 weights
-// of a tile 2048 cycles of it.
-__device__ __forceinline__ void ex2_cubic(float& x0, float& x1) {
-  float p0, p1, n0, n1;
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x0));      // -127; what is no number stays so
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x1));
-  asm("{\n .reg .b64 x, n, f, p, c;\n mov.b64 x, {%4, %5};\n mov.b64 c, {%6, %6};\n add.rn.f32x2 n, x, c;\n mov.b64 {%2, %3}, n;\n"
-      " mov.b64 c, {%7, %7};\n add.rn.f32x2 f, n, c;\n mov.b64 c, {%8, %8};\n fma.rn.f32x2 f, f, c, x;\n"
-      " mov.b64 p, {%9, %9};\n mov.b64 c, {%10, %10};\n fma.rn.f32x2 p, p, f, c;\n mov.b64 c, {%11, %11};\n fma.rn.f32x2 p, p, f, c;\n"
-      " mov.b64 c, {%12, %12};\n fma.rn.f32x2 p, p, f, c;\n mov.b64 {%0, %1}, p;\n}\n"
-      : "=f"(p0), "=f"(p1), "=f"(n0), "=f"(n1)
-      : "f"(x0), "f"(x1), "f"(12582912.f), "f"(-12582912.f), "f"(-1.f), "f"(0.055008747f), "f"(0.24221076f), "f"(0.69328290f), "f"(1.f));
-  x0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
-  x1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
-}
-
 // Bits of the keys key0 .. key0 + 31 that a row sees: of the context from `begin` on, of the new ones by the token's mask (and the window).
 // near: the mask's first 64 bits.
 __device__ __forceinline__ uint32_t seen_bits(const Args& a, const Item& it, int key0, int begin, const int* mask, uint64_t near) {
@@ -306,7 +289,6 @@ __global__ void __launch_bounds__(threads_of(SETS), 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const Tc k) {
   constexpr int SOFTMAX_WARPS = 4 * SETS, PRODUCER_WARP = SOFTMAX_WARPS, MMA_WARP = SOFTMAX_WARPS + 1;
   constexpr int N = 64;                                 // scores in registers at a time; their weights lie over the first half of them
-  constexpr int CUBIC = 1, CUBIC_OF = 4;                // pairs of weights of each four that are made without the exponential unit
   constexpr int COL_BYTES = BN * 128, Q_COL_BYTES = BM * 128;
   const Args& a = k.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -630,12 +612,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
           const int u = u0 + value_unit(j, tiles), turn = u / k.ring, unit = u - turn * k.ring;
           mbar_wait(&u_full[unit], (uint32_t)(turn & 1), abort, k.status);
           unsigned char* v_s = ring_s + unit * unit_bytes;
-          constexpr int STEP = KEYS ? BM : 32 * SOFTMAX_WARPS;
-          const int at0 = KEYS ? r : threadIdx.x;
           const __nv_bfloat162 nought = __floats2bfloat162_rn(0.f, 0.f);
           __nv_bfloat162 sum = nought;      // 0 x of all of them: a NaN where one is not finite
 #pragma unroll 4
-          for (int i = at0; i < unit_bytes / 16; i += STEP) {
+          for (int i = r; i < unit_bytes / 16; i += BM) {
             const uint4 x = *reinterpret_cast<const uint4*>(v_s + 16 * i);
             sum = __hfma2(reinterpret_cast<const __nv_bfloat162&>(x.x), nought, sum);
             sum = __hfma2(reinterpret_cast<const __nv_bfloat162&>(x.y), nought, sum);
@@ -643,92 +623,78 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
             sum = __hfma2(reinterpret_cast<const __nv_bfloat162&>(x.w), nought, sum);
           }
           if (__low2float(sum) != 0.f || __high2float(sum) != 0.f) {
-            for (int i = at0; i < unit_bytes / 16; i += STEP) {
+            spoiled[it & 1] = it + 1;      // (first: two sets of rows on the same tile may find the other's zeros instead)
+            __threadfence_block();
+            for (int i = r; i < unit_bytes / 16; i += BM) {
               uint4 x = *reinterpret_cast<const uint4*>(v_s + 16 * i);
               uint32_t* w4 = &x.x;
 #pragma unroll
               for (int e = 0; e < 4; ++e) w4[e] &= ~__vcmpeq2(w4[e] & 0x7f807f80u, 0x7f807f80u);
               *reinterpret_cast<uint4*>(v_s + 16 * i) = x;
             }
-            spoiled[it & 1] = it + 1;
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          if constexpr (KEYS) {
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + set), "n"(BM) : "memory");      // the tile is this set's alone
-          } else {
-            sync_softmax();
-          }
+          asm volatile("bar.sync %0, %1;" ::"r"(1 + set), "n"(BM) : "memory");
         }
         if (busy) {
-          float v[N];
-          auto scores_at = [&](int col) {      // of this thread's columns col .. col + N - 1, -infinity where the row may not see the key
-            tmem_ld(v, s_addr + col);
-            if (a.softcap > 0.f) {
-#pragma unroll
-              for (int e = 0; e < N; ++e) v[e] = mi::shaped_logit2(v[e], a.scale, a.softcap, false, 0.f);
-            }
-            if (masked) {
-#pragma unroll
-              for (int e = 0; e < N; ++e) v[e] = (bits[(col + e) / 32] >> (e & 31)) & 1 ? v[e] : -INFINITY;
-            }
-          };
-          auto largest = [&]() {
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < N; e += 2) mx4[e >> 1 & 3] = mi::max_of(mx4[e >> 1 & 3], v[e], v[e + 1]);
-            return fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-          };
-          scores_at(0);
-          float mx = largest();
-          if constexpr (BN > N) {
-            scores_at(N);
-            mx = fmaxf(mx, largest());
-          }
-          const float m_new = fmaxf(m_run, mx * factor);      // the scale is positive
-          const bool move = m_new > m_run + 8.f;      // (of the first key: from -infinity)
-          if (__any_sync(0xffffffffu, move)) {
-            const float alpha = move ? exp2f(m_run - m_new) : 1.f;
-            if (!first_of_set) {      // (its last P V is done: this tile's scores came behind it)
+          // The first scores, the last ones - which stay in registers -, and once the maximum is known the first again: one piece of code three times, for
+          // what runs a few times a block is bound by fetching its instructions.
+          constexpr int CHUNKS = BN / N;
+          float v[N], mx = -INFINITY, m_use = 0.f, part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-              for (int c = 0; 16 * c < k.n_out; ++c) {      // (16 at a time: the scores are in registers too)
-                float o[16];
-                uint32_t x[16];
-                tmem_ld(o, o_addr + 16 * c);
+          for (int step = 0; step < 2 * CHUNKS - 1; ++step) {
+            const int col = step == 1 ? N : 0;
+            tmem_ld(v, s_addr + col);
+            if (a.softcap > 0.f) {      // cap tanh(x / cap) in base 2, as cap (1 - 2 / (1 + e^(2 x / cap))); beyond the bound tanh is 1 to the last bit
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                  mi::mul_pair(o[e], o[e + 1], o[e], o[e + 1], alpha);
-                  x[e] = __float_as_uint(o[e]);
-                  x[e + 1] = __float_as_uint(o[e + 1]);
-                }
-                tmem_st(o_addr + 16 * c, x);
-              }
+              for (int e = 0; e < N; ++e) v[e] = k.cap_log2 - __fdividef(2.f * k.cap_log2, 1.f + mi::ex2_fast(fminf(v[e] * k.cap_scale, 60.f)));
             }
-            l_run *= alpha;
-            if (move) m_run = m_new;
-          }
-          const float m_use = m_run == -INFINITY ? 0.f : m_run;
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-          auto weigh = [&](int col) {      // over its own scores, two keys to a column
+            if (masked) {      // -infinity where the row may not see the key
+              const uint32_t b0 = step == 1 ? bits[BN / 32 - 2] : bits[0], b1 = step == 1 ? bits[BN / 32 - 1] : bits[1];
+#pragma unroll
+              for (int e = 0; e < N; ++e) v[e] = ((e < 32 ? b0 : b1) >> (e & 31)) & 1 ? v[e] : -INFINITY;
+            }
+            if (step < CHUNKS) {
+              float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int e = 0; e < N; e += 2) mx4[e >> 1 & 3] = mi::max_of(mx4[e >> 1 & 3], v[e], v[e + 1]);
+              mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+            }
+            if (step < CHUNKS - 1) continue;
+            if (step == CHUNKS - 1) {
+              const float m_new = fmaxf(m_run, mx * factor);      // the scale is positive
+              const bool move = m_new > m_run + 8.f;      // (of the first key: from -infinity)
+              if (__any_sync(0xffffffffu, move)) {
+                const float alpha = move ? exp2f(m_run - m_new) : 1.f;
+                if (!first_of_set) {      // (its last P V is done: this tile's scores came behind it)
+#pragma unroll 1
+                  for (int c = 0; 16 * c < k.n_out; ++c) {      // (16 at a time: the scores are in registers too)
+                    float o[16];
+                    uint32_t x[16];
+                    tmem_ld(o, o_addr + 16 * c);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                      mi::mul_pair(o[e], o[e + 1], o[e], o[e + 1], alpha);
+                      x[e] = __float_as_uint(o[e]);
+                      x[e + 1] = __float_as_uint(o[e + 1]);
+                    }
+                    tmem_st(o_addr + 16 * c, x);
+                  }
+                }
+                l_run *= alpha;
+                if (move) m_run = m_new;
+              }
+              m_use = m_run == -INFINITY ? 0.f : m_run;
+            }
             uint32_t packed[N / 2];
 #pragma unroll
             for (int e = 0; e < N; e += 2) mi::fma_pair(v[e], v[e + 1], v[e], v[e + 1], factor, -m_use);
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
-              if (e % CUBIC_OF < CUBIC) {
-                ex2_cubic(v[2 * e], v[2 * e + 1]);
-              } else {
-                v[2 * e] = mi::ex2_fast(v[2 * e]);
-                v[2 * e + 1] = mi::ex2_fast(v[2 * e + 1]);
-              }
-              packed[e] = pack_bf16(v[2 * e], v[2 * e + 1]);      // nothing where the row may not see the key
+              packed[e] = pack_bf16(mi::ex2_fast(v[2 * e]), mi::ex2_fast(v[2 * e + 1]));      // nothing where the row may not see the key
               mi::add_pair(part[2 * e & 3], part[(2 * e + 1) & 3], __uint_as_float(packed[e] << 16), __uint_as_float(packed[e] & 0xffff0000u));
             }
-            tmem_st(s_addr + col, packed);
-          };
-          weigh(BN - N);      // the last scores are still in registers, the first are read again
-          if constexpr (BN > N) {
-            scores_at(0);
-            weigh(0);
+            tmem_st(s_addr + col, packed);      // two keys to a column, over the first half of their scores
           }
           l_run += (part[0] + part[1]) + (part[2] + part[3]);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -742,7 +708,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         mbar_wait(&o_full[set], (g - 1) & 1, abort, k.status);
         tc_fence_after();
       }
-      if (!(l_run < 1e30f)) l_run = __int_as_float(0x7fffffff);      // a score that is no number (ex2_cubic makes a huge weight of it)
       float m_all = m_run, l_all = l_run, scale0 = 1.f, scale1 = 0.f;
       if constexpr (KEYS) {      // the two streams' sums of this row
         of_set[set * BM + r] = make_float2(m_run, l_run);
@@ -958,6 +923,8 @@ MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, cons
   k.tokens = BM / G;
   k.max_parts = (max_q + qt * k.tokens - 1) / (qt * k.tokens);
   k.scale_log2 = scale * 1.4426950408889634f;
+  k.cap_log2 = softcap * 1.4426950408889634f;
+  k.cap_scale = softcap > 0.f ? 2.f * k.scale_log2 / softcap : 0.f;
   const int blocks = mi::sm_count();
   k.joins = (int4*)scratch;
   float* part_o = scratch + 4ll * blocks;
