@@ -32,11 +32,12 @@ constexpr int TMEM_COLS = 512, S_COL = 256;
 constexpr int MAX_UNITS = 12;                 // boxes of the ring: a tile's keys or its values each
 constexpr int WAIT_LIMIT = 1 << 22;
 constexpr int SMEM_BYTES = 227 << 10;
-constexpr int BARS = 76;                      // 8-byte words behind queries and ring: barriers, pieces
+constexpr int BARS = 80;                      // 8-byte words behind queries and ring: barriers, pieces
 
 struct Tc {
   Args a;
   int* status;
+  int* counters;                 // [items * nkv * max_parts], zero, left zero: pieces of a unit that have come; null: tree_join_kernel joins them
   int4* joins;                   // [blocks]: of the unit that begins in a block and goes on in others: pieces, first token, tokens, key/value head
   int boxes, steps, n_out;       // boxes and 16s of columns of a row, columns of P V
   int ring, box_rows;            // units of the ring; rows of a TMA box of keys
@@ -194,7 +195,7 @@ struct Piece {
   int n, key;                    // tiles (0: no piece is left), first key
   int head, first;               // key/value head; the unit's first token in the item
   int slot;                      // of the sums, where the unit goes on in other blocks; -1: it does not
-  int pieces;                    // where it begins here and goes on: in how many blocks; else 0
+  int unit, block, pieces;       // the unit's number, its first block, in how many blocks it lies
 };
 constexpr int PIECES = 4;        // that are described at a time: the producer is at most two ahead of the last reader
 
@@ -229,7 +230,9 @@ struct Walk {
       const int part = unit - p.head * l.parts;
       p.first = part * QT * k.tokens;
       p.slot = p.n == l.tiles ? -1 : 2 * (int)blockIdx.x + (j0 == 0 ? 1 : 0);
-      p.pieces = p.n < l.tiles && j0 == 0 ? stretch_of(base, more, first_tile + l.tiles - 1) - (int)blockIdx.x + 1 : 0;
+      p.unit = (item * k.a.nkv + p.head) * k.max_parts + part;
+      p.block = p.n == l.tiles ? (int)blockIdx.x : stretch_of(base, more, first_tile);
+      p.pieces = p.n == l.tiles ? 1 : stretch_of(base, more, first_tile + l.tiles - 1) - p.block + 1;
       return true;
     }
     return false;
@@ -282,6 +285,65 @@ __device__ __forceinline__ void add_not_finite(const Args& a, const Item& it, in
   }
 }
 
+// Row r of set `set` of a unit that lies in u.x blocks from `first` on - its first token u.y, tokens u.z, key/value head u.w -, columns 4 f0 .. 4 (f0 + F) - 1: the
+// pieces' sums added up.  Piece s lies in block first + s: as that block's second of the sums where the unit begins there, else as its first.
+template <int QT, int F, int AT_ONCE>
+__device__ __forceinline__ void join_row(const Tc& k, int first, const int4& u, int set, int r, int f0) {
+  const Args& a = k.a;
+  const int row = set * BM + r, pieces = u.x, token = u.y + set * k.tokens + r / a.G, h = u.w * a.G + r % a.G;
+  if (r >= min(k.tokens, u.z - set * k.tokens) * a.G || 4 * f0 >= a.hd) return;
+  const float2* sums = reinterpret_cast<const float2*>(a.part_ml) + row;
+  const float4* values = reinterpret_cast<const float4*>(a.part_o) + (size_t)f0 * (QT * BM) + row;
+  const float sink2 = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
+  float top = sink2, total = a.sink ? 1.f : 0.f;
+  float acc[F][4] = {};
+#pragma unroll 1
+  for (int s0 = 0; s0 < pieces; s0 += AT_ONCE) {
+    float2 ml[AT_ONCE];
+    float4 x[AT_ONCE][F];
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s) {
+      ml[s] = make_float2(-INFINITY, 0.f);
+      const size_t at = 2 * (first + s0 + s) + (s0 + s == 0 ? 1 : 0);
+      if (s0 + s < pieces) ml[s] = __ldcg(sums + at * (QT * BM));
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        x[s][f] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s0 + s < pieces) x[s][f] = __ldcg(values + (at * (k.n_out / 4) + f) * (QT * BM));
+      }
+    }
+    float next = top;
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s) next = fmaxf(next, ml[s].x);
+    const float off = next == -INFINITY ? 0.f : next, alpha = exp2f(top - off);
+    top = next;
+    total *= alpha;
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[f][e] *= alpha;
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s) {
+      const float w = exp2f(ml[s].x - off);
+      total = fmaf(ml[s].y, w, total);
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        acc[f][0] = fmaf(x[s][f].x, w, acc[f][0]);
+        acc[f][1] = fmaf(x[s][f].y, w, acc[f][1]);
+        acc[f][2] = fmaf(x[s][f].z, w, acc[f][2]);
+        acc[f][3] = fmaf(x[s][f].w, w, acc[f][3]);
+      }
+    }
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;      // nothing visible: zeros
+  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)token * a.nh + h) * a.hd + 4 * f0;
+#pragma unroll
+  for (int f = 0; f < F; f += 2)      // (a head size is a multiple of 16)
+    if (4 * (f0 + f) < a.hd)
+      *reinterpret_cast<uint4*>(dst + 4 * f) = make_uint4(pack_bf16(acc[f][0] * inv, acc[f][1] * inv), pack_bf16(acc[f][2] * inv, acc[f][3] * inv),
+                                                          pack_bf16(acc[f + 1][0] * inv, acc[f + 1][1] * inv), pack_bf16(acc[f + 1][2] * inv, acc[f + 1][3] * inv));
+}
+
 constexpr int threads_of(int sets) { return 32 * (4 * sets + 2); }
 
 template <int QT, int SETS, int BN, int STEPS>
@@ -311,6 +373,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + BUFFERS);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* spoiled = abort + 1;      // [2]: the last piece, by parity, in which a value was not finite
+  volatile int* last_to_come = spoiled + 2;
   Piece* pieces = reinterpret_cast<Piece*>(bars + 44);
   float2* of_set = reinterpret_cast<float2*>(bars + BARS);      // [2][BM]: a row's maximum and sum in each stream of keys, at a piece's end
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -417,7 +480,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       }
       if (!more_pieces) break;
       if (lane == 0) {
-        if (p.pieces) joined = make_int4(p.pieces, p.it.row0 + p.first, min(p.it.n - p.first, QT * k.tokens), p.head);
+        if (p.pieces > 1 && p.block == me) joined = make_int4(p.pieces, p.it.row0 + p.first, min(p.it.n - p.first, QT * k.tokens), p.head);
         mbar_expect_tx(q_full, (uint32_t)(QT * k.boxes * rows * 128));
         for (int s = 0; s < QT; ++s)
           for (int c = 0; c < k.boxes; ++c)
@@ -771,6 +834,23 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
+      if (QT == 1 && !whole && k.counters) {      // few rows: the unit's last piece to come joins them all, a launch less
+        __threadfence();
+        sync_softmax();
+        if (threadIdx.x == 0) {
+          const bool all = atomicAdd(k.counters + p.unit, 1) == p.pieces - 1;
+          if (all) k.counters[p.unit] = 0;      // ready for the next launch
+          *last_to_come = all;
+        }
+        sync_softmax();
+        if (*last_to_come) {
+          __threadfence();
+          const int4 u = make_int4(p.pieces, p.it.row0 + p.first, min(p.it.n - p.first, k.tokens), p.head);
+          const int quarters = (min(k.tokens, u.z) * a.G + 31) / 32;      // a warp 32 rows and 8 columns at a time
+#pragma unroll 1
+          for (int w = warp; w < quarters * (k.n_out / 8); w += SOFTMAX_WARPS) join_row<1, 2, 8>(k, p.block, u, 0, w % quarters * 32 + lane, w / quarters * 2);
+        }
+      }
       u0 = (u0 + 2 * tiles) % (2 * k.ring);      // (as far as slot and parity go)
     }
   }
@@ -784,69 +864,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
   }
 }
 
-// The pieces of units that several blocks shared, added up: for the unit that begins in a block and goes on in others, grid (blocks, QT, columns / (4 F
-// JOIN_WARPS / 4)); a lane a row and 4 F columns, a warp 32 rows.  Piece s lies in block first + s: as that block's second of the sums where the unit
-// begins there, else as its first.  AT_ONCE pieces are on their way at a time, their maxima and sums with them.
+// The pieces of units that several blocks shared, where the last block to come does not join them: for the unit that begins in a block and goes on in others,
+// grid (blocks, QT, columns / (4 F JOIN_WARPS / 4)); a lane a row and 4 F columns, a warp 32 rows, AT_ONCE pieces on their way at a time.
 constexpr int JOIN_WARPS = 8;
 template <int QT, int F, int AT_ONCE>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
 tree_join_kernel(const Tc k) {
-  const Args& a = k.a;
-  const int warp = threadIdx.x >> 5, set = blockIdx.y, r = warp % 4 * 32 + (threadIdx.x & 31), f0 = (blockIdx.z * (JOIN_WARPS / 4) + warp / 4) * F, row = set * BM + r;
+  const int warp = threadIdx.x >> 5;
   mi::grid_dependency_sync();
   const int4 u = k.joins[blockIdx.x];
-  const int first = (int)blockIdx.x, pieces = u.x, token = u.y + set * k.tokens + r / a.G, h = u.w * a.G + r % a.G;
-  if (pieces == 0 || r >= min(k.tokens, u.z - set * k.tokens) * a.G || 4 * f0 >= a.hd) return;
-  const float2* sums = reinterpret_cast<const float2*>(a.part_ml) + row;
-  const float4* values = reinterpret_cast<const float4*>(a.part_o) + (size_t)f0 * (QT * BM) + row;
-  const float sink2 = a.sink ? a.sink[h] * 1.4426950408889634f : -INFINITY;
-  float top = sink2, total = a.sink ? 1.f : 0.f;
-  float acc[F][4] = {};
-#pragma unroll 1
-  for (int s0 = 0; s0 < pieces; s0 += AT_ONCE) {
-    float2 ml[AT_ONCE];
-    float4 x[AT_ONCE][F];
-#pragma unroll
-    for (int s = 0; s < AT_ONCE; ++s) {
-      ml[s] = make_float2(-INFINITY, 0.f);
-      const size_t at = 2 * (first + s0 + s) + (s0 + s == 0 ? 1 : 0);
-      if (s0 + s < pieces) ml[s] = sums[at * (QT * BM)];
-#pragma unroll
-      for (int f = 0; f < F; ++f) {
-        x[s][f] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s0 + s < pieces) x[s][f] = values[(at * (k.n_out / 4) + f) * (QT * BM)];
-      }
-    }
-    float next = top;
-#pragma unroll
-    for (int s = 0; s < AT_ONCE; ++s) next = fmaxf(next, ml[s].x);
-    const float off = next == -INFINITY ? 0.f : next, alpha = exp2f(top - off);
-    top = next;
-    total *= alpha;
-#pragma unroll
-    for (int f = 0; f < F; ++f)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[f][e] *= alpha;
-#pragma unroll
-    for (int s = 0; s < AT_ONCE; ++s) {
-      const float w = exp2f(ml[s].x - off);
-      total = fmaf(ml[s].y, w, total);
-#pragma unroll
-      for (int f = 0; f < F; ++f) {
-        acc[f][0] = fmaf(x[s][f].x, w, acc[f][0]);
-        acc[f][1] = fmaf(x[s][f].y, w, acc[f][1]);
-        acc[f][2] = fmaf(x[s][f].z, w, acc[f][2]);
-        acc[f][3] = fmaf(x[s][f].w, w, acc[f][3]);
-      }
-    }
-  }
-  const float inv = total == 0.f ? 0.f : 1.f / total;      // nothing visible: zeros
-  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)token * a.nh + h) * a.hd + 4 * f0;
-#pragma unroll
-  for (int f = 0; f < F; f += 2)      // (a head size is a multiple of 16)
-    if (4 * (f0 + f) < a.hd)
-      *reinterpret_cast<uint4*>(dst + 4 * f) = make_uint4(pack_bf16(acc[f][0] * inv, acc[f][1] * inv), pack_bf16(acc[f][2] * inv, acc[f][3] * inv),
-                                                          pack_bf16(acc[f + 1][0] * inv, acc[f + 1][1] * inv), pack_bf16(acc[f + 1][2] * inv, acc[f + 1][3] * inv));
+  if (u.x) join_row<QT, F, AT_ONCE>(k, blockIdx.x, u, blockIdx.y, warp % 4 * 32 + (threadIdx.x & 31), (blockIdx.z * (JOIN_WARPS / 4) + warp / 4) * F);
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -876,6 +903,10 @@ int launch(Tc& k, const CUtensorMap& q_map, const CUtensorMap& kv_map, int block
   MI_REQUIRE(k.ring >= 4, "attention_tree_tc: no room for a ring of tiles of %d boxes", k.boxes);
   if (mi::launch(tree_tc_kernel<QT, SETS, BN, STEPS>, dim3(blocks), dim3(threads_of(SETS)), SMEM_BYTES, stream, q_map, kv_map, k) != cudaSuccess)
     return mi_fail("attention_tree_tc: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  if (k.counters) {
+    MI_LAUNCH_OK("attention_tree_tc");
+    return 0;
+  }
   // Many pieces of a unit where there are fewer units than blocks: eight at a time of 8 columns; else two at a time of 32.
   const Args& a = k.a;
   const bool few = (long long)a.items * a.nkv * k.max_parts < blocks;
@@ -886,6 +917,9 @@ int launch(Tc& k, const CUtensorMap& q_map, const CUtensorMap& kv_map, int block
   MI_LAUNCH_OK("attention_tree_tc");
   return 0;
 }
+
+// (8 rows in 20 pieces a unit, 164 KB: 16.6 us on the device either way, and 5 us less to launch; 96 rows in 4 pieces, 256 KB: 31 against 24 us)
+constexpr long long JOIN_INSIDE_BYTES = 192 << 10;
 
 // Sets of 128 rows that a block takes at a time: two once the largest item has more rows than one holds, as far as tensor memory goes.
 int sets_of(int max_q, int G, int hd) { return hd <= 128 && max_q > BM / G ? 2 : 1; }
@@ -899,11 +933,12 @@ MI_API long long mi_attention_tree_tc_floats(int nh, int nkv, int hd, int page_s
   return 4 * blocks + 2 * blocks * sets_of(max_q, nh / nkv, hd) * BM * ((hd + BOX - 1) / BOX * BOX + 2);
 }
 
-// bfloat16.  scratch: mi_attention_tree_tc_floats floats, 16-byte aligned; status: one word, set to 2 if a bounded wait ran out, to 4 if shared memory is
+// bfloat16.  scratch: mi_attention_tree_tc_floats floats, 16-byte aligned; counters: a zero word for each item, key/value head and set of
+// 128 / G tokens of max_q, left zero; status: one word, set to 2 if a bounded wait ran out, to 4 if shared memory is
 // not laid out as the kernel needs it.  Answers 2 for sizes or addresses that it does not take.
 MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, const int* block_table, int bt_stride, const int* q_start, const int* q_len,
                                 const int* ctx_len, const int* seq_slot, const int* mask, int words, const int* positions, const float* sink, float* scratch,
-                                int* status, int items, int T, int width, int nh, int nkv, int hd, int pages, int page_size, int window, int max_q, float scale,
+                                int* counters, int* status, int items, int T, int width, int nh, int nkv, int hd, int pages, int page_size, int window, int max_q, float scale,
                                 float softcap, cudaStream_t stream) {
   MI_REQUIRE(items >= 0 && T >= 0 && nkv > 0 && nh % nkv == 0 && bt_stride > 0 && pages > 0 && (long long)words * 32 >= max_q, "attention_tree_tc: bad sizes items=%d T=%d words=%d max_q=%d", items, T, words, max_q);
   if (mi_attention_tree_tc_floats(nh, nkv, hd, page_size, max_q) == 0 || width % 8 != 0 || !(scale > 0.f) || T == 0 ||
@@ -926,6 +961,9 @@ MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, cons
   k.cap_log2 = softcap * 1.4426950408889634f;
   k.cap_scale = softcap > 0.f ? 2.f * k.scale_log2 / softcap : 0.f;
   const int blocks = mi::sm_count();
+  // Pieces are joined by the unit's last block to come, a launch less, where that is little for one block to do; else by a kernel of their own.
+  const long long units = (long long)items * nkv * k.max_parts, rows = (long long)max_q * G, pieces = blocks / units + 2;
+  k.counters = qt == 1 && rows <= BM && pieces * rows * hd * 4 <= JOIN_INSIDE_BYTES ? counters : nullptr;
   k.joins = (int4*)scratch;
   float* part_o = scratch + 4ll * blocks;
   float* part_ml = part_o + 2ll * blocks * qt * BM * k.n_out;

@@ -1688,13 +1688,16 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
   stream = _current_stream(device)
   n = _tree_tc_floats(num_heads, num_kv_heads, head_dim, page_size, max_q) if dt == BF16 else 0
   if n:
+    # counters of a unit's pieces: an item, a key/value head and as many tokens as 128 rows hold
+    units = batch.num_items * num_kv_heads * -(-max_q // (128 // (num_heads // num_kv_heads)))
     if ws is not None:
-      scratch, status = ws.buffer("attention_tree_partials", (n,), torch.float32), ws.zeros("attention_tree_status", 1, torch.int32)
+      scratch = ws.buffer("attention_tree_partials", (n,), torch.float32)
+      counters, status = ws.zeros("attention_tree_counters", units, torch.int32), ws.zeros("attention_tree_status", 1, torch.int32)
     else:
       scratch = torch.empty(n, dtype=torch.float32, device=qkv.device)
-      status = torch.zeros(1, dtype=torch.int32, device=qkv.device)
-    code = _entry("mi_attention_tree_tc", "ppppi" + "ppppp" + "ippppi" + "iiiiiiiiiffp")(
-      *head, *where, scratch.data_ptr(), status.data_ptr(), *sizes, stream)
+      counters, status = torch.zeros(units, dtype=torch.int32, device=qkv.device), torch.zeros(1, dtype=torch.int32, device=qkv.device)
+    code = _entry("mi_attention_tree_tc", "ppppi" + "ppppp" + "ipppppi" + "iiiiiiiiiffp")(
+      *head, *where, scratch.data_ptr(), counters.data_ptr(), status.data_ptr(), *sizes, stream)
     if code != TREE_NOT_TAKEN:
       _check(common_lib(), code, kernels=2)
       if ws is None and int(status[0]) != 0:
