@@ -13,7 +13,7 @@
 //
 // The n best of a tile without sorting it: a thread's best of its own 16, and of each warp's 32 the ceil(n / 8)-th - eight warps make n of them -; the
 // least of these eight bounds the tile's n-th best from below.  What is not below it - 2 or 3 n, as a rule - is collected in shared memory and ranked
-// by counting.  Should more come than there is room for (many equal values, a tile of which a warp has only poor ones), the n-th best of the 256 threads'
+// by counting.  Should many more come (equal values, a tile of which a warp has only poor ones or none), the n-th best of the 256 threads'
 // bests is found exactly: at most n times a thread's 16 values are not below that.
 //
 // Float32 holds a value and a piece's sum; normalisers and scores are made in 64 bits, so that candidates of different beams, which may lie
@@ -27,7 +27,8 @@ constexpr int THREADS = 256, WARPS = THREADS / 32, ITEMS = 16, TILE = THREADS * 
 constexpr int STAGES = 4;                     // tiles in shared memory: three on their way, one that was just read
 constexpr int MAX_BEST = 128;
 constexpr int ROOM = MAX_BEST * (ITEMS + 1) + 384;      // candidates: the n best so far and a tile's on top; what is over lets a few tiles come before they are thinned out
-constexpr int BLOCKS_WANTED = 1;
+constexpr int BLOCKS_WANTED = 1;              // (64 requests, 263 rows: 48 us; 2, which are one and a half rounds of blocks: 63)
+constexpr int MANY = 256;                     // candidates of a tile that are ranked without a second thought
 constexpr unsigned FULL = 0xffffffffu;
 
 // Rises with the value; minus and plus zero are one.  (Values that are no numbers never come here.)
@@ -461,28 +462,30 @@ beam_select_kernel(Args a) {
         return key_of(mi::to_float(x[token]), token);
       }
     };
-    const bool bounded = most + beating * ITEMS > ROOM;
+    const bool bounded = t == 0 || most + beating * ITEMS > ROOM;      // (the first tile has no bar: all of a small vocabulary would be ranked)
     if (bounded) {
       const int before = s_count;
       const uint32_t high = top > -INFINITY ? rising(top) : 0;
       uint64_t bound = (uint64_t)quick_bound(high, a.n, of_warp) << 32;
 #pragma unroll 1
       for (bool again = false;; again = true) {
-        uint32_t mine = hits;
+        const float least = bound ? value_of(bound) : -INFINITY;
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) mine |= (v[j] >= least ? 1u : 0u) << j;
+        mine &= hits;
 #pragma unroll 1
-        for (uint32_t todo = hits; todo; todo &= todo - 1)
+        for (uint32_t todo = mine; todo; todo &= todo - 1)      // (of equal values the lower tokens)
           if (key_by_number(__ffs(todo) - 1) < bound) mine &= ~(todo & -todo);
         int i = mine ? atomicAdd(&s_count, __popc(mine)) : 0;
 #pragma unroll 1
         for (; mine && i < ROOM; mine &= mine - 1) pool[i++] = key_by_number(__ffs(mine) - 1);
         __syncthreads();
-        if (again || s_count <= ROOM) break;
-        uint64_t best = 0;      // more than there is room for: the exact bound of the threads' bests
-#pragma unroll 1
-        for (uint32_t todo = hits; todo; todo &= todo - 1) {
-          const uint64_t key = key_by_number(__ffs(todo) - 1);
-          best = key > best ? key : best;
-        }
+        if (again || s_count - before <= MANY) break;
+        uint64_t best = 0;      // more than are ranked in a moment: the exact bound of the threads' bests
+#pragma unroll
+        for (int j = ITEMS - 1; j >= 0; --j)
+          if (v[j] == top && top > bar) best = key_of(top, token_at<T, WIDE>(begin, j));
         bound = nth_best(best, a.n, lists, &s_nth);
         if (threadIdx.x == 0) s_count = before;
         __syncthreads();
@@ -493,7 +496,7 @@ beam_select_kernel(Args a) {
       for (; hits; hits &= hits - 1) pool[i++] = key_by_number(__ffs(hits) - 1);
     }
     most = bounded ? ROOM : most + beating * ITEMS;
-    if ((t & (t + 1)) == 0) {      // tiles 0, 1, 3, 7, ..: the bar rises as fast as the tiles say less
+    if (t == 0 || t == 3 || t == 15) {      // the bar rises as the tiles say less
       __syncthreads();
       thin_out();
       most = a.n;
@@ -556,7 +559,7 @@ int launch(const Args& a, cudaStream_t stream) {
 
 }  // namespace
 
-// Tiles of a block's stretch: as many as leave BLOCKS_WANTED blocks an SM (two fit at a time).
+// Tiles of a block's stretch: as many as leave BLOCKS_WANTED blocks an SM (two fit at a time), a block a row at least.
 static int beam_tiles(int R, int V) {
   const long long tiles = ((long long)V + TILE - 1) / TILE, wanted = (long long)BLOCKS_WANTED * mi::sm_count();
   const long long stretches = R > 0 ? (wanted + R - 1) / R : 1;

@@ -156,3 +156,26 @@ def test_captured_and_replayed_with_a_shared_workspace():
       graph.replay()
     for _, out, logits, cum, starts, start, n in calls:
       check(out, logits, cum, start, n)
+
+
+def test_on_a_stream_of_its_own():
+  if DEV == "cpu":
+    pytest.skip("streams")
+  logits, cum = torch.randn((6, 20000), device=DEV), torch.zeros(6, device=DEV)
+  want = select(logits, cum, [0, 2, 6], 12)
+  torch.cuda.synchronize()
+  side = torch.cuda.Stream()
+  with torch.cuda.stream(side):
+    got = select(logits, cum, [0, 2, 6], 12)
+  side.synchronize()
+  assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("start", [[0, 2, 5], [1, 3, 3, 4], [3, 8], [0, 0, 0]])
+def test_rows_of_no_request_and_lists_that_end_behind_the_rows(start):
+  """Rows in front of the first request and behind the last belong to nobody; a list that goes on past the rows is cut."""
+  g = torch.Generator().manual_seed(sum(start))
+  logits, cum = torch.randn((5, 6000), generator=g).to(DEV), torch.zeros(5, device=DEV)
+  cut = [min(s, 5) for s in start]
+  for _ in range(2):      # (the second call finds the counters as the first left them)
+    check(select(logits, cum, start, 7), logits, cum, cut, 7)

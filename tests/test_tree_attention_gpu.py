@@ -159,3 +159,20 @@ def test_on_a_stream_of_its_own():
     ops.tree_attention(got, *args)
   side.synchronize()
   assert torch.equal(want, got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_pages_beyond_32_bits_of_a_cache(dtype):
+  """The last pages of a layer's cache of more than 2^31 values."""
+  from miniinfer_b200.kernels import ops
+  if DEV == "cpu":
+    pytest.skip("memory")
+  qkv, kv, table, batch = tree_case([(300, 20), (70, 3)], 16, 8, 128, 64, dtype, seed=9)
+  want = torch.empty((qkv.shape[0], 16 * 128), dtype=dtype, device=DEV)
+  ops.tree_attention(want, qkv, kv, table, batch, 16, 8, 128, 128 ** -0.5)
+  pages = (1 << 31) // kv[0].numel() + kv.shape[0] + 1
+  large = torch.zeros((pages,) + kv.shape[1:], dtype=dtype, device=DEV)
+  large[-kv.shape[0]:] = kv
+  got = torch.empty_like(want)
+  ops.tree_attention(got, qkv, large, table + (pages - kv.shape[0]), batch, 16, 8, 128, 128 ** -0.5)
+  assert torch.equal(got, want)
