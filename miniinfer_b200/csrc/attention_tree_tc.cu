@@ -708,9 +708,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
           for (int step = 0; step < 2 * CHUNKS - 1; ++step) {
             const int col = step == 1 ? N : 0;
             tmem_ld(v, s_addr + col);
-            if (a.softcap > 0.f) {      // cap tanh(x / cap) in base 2, as cap (1 - 2 / (1 + e^(2 x / cap))); beyond the bound tanh is 1 to the last bit
+            if (a.softcap > 0.f) {      // cap tanh(x / cap) in base 2, as cap (1 - 2 / (1 + e^(2 x / cap))): 0 is taken off where the sum is infinite
 #pragma unroll
-              for (int e = 0; e < N; ++e) v[e] = k.cap_log2 - __fdividef(2.f * k.cap_log2, 1.f + mi::ex2_fast(fminf(v[e] * k.cap_scale, 60.f)));
+              for (int e = 0; e < N; ++e) v[e] = k.cap_log2 - __fdividef(2.f * k.cap_log2, 1.f + mi::ex2_fast(v[e] * k.cap_scale));
             }
             if (masked) {      // -infinity where the row may not see the key
               const uint32_t b0 = step == 1 ? bits[BN / 32 - 2] : bits[0], b1 = step == 1 ? bits[BN / 32 - 1] : bits[1];

@@ -96,6 +96,32 @@ def test_numbers_that_are_not_finite_reach_only_rows_that_see_them(dtype, bad):
           assert torch.isfinite(heads[t][:, other]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_cap_hides_infinite_scores_and_no_scores_that_are_no_numbers(hd, dtype):
+  """Scores far beyond the cap, and infinite ones, are the cap; a key that holds a NaN makes the rows NaN that see it."""
+  from miniinfer_b200.kernels import ops
+  case = ([(130, 12)], 8, 2, hd, 64, None, False, 5.0, 0.0)
+  clean, args = run(case, dtype)
+  qkv, kv, table, batch = args[:4]
+  node, place = 4, 130 + 4
+  sees = [bool(m >> node & 1) for m in batch.tree_mask[:, 0].tolist()]
+  assert any(sees) and not all(sees)
+  page = int(table[int(batch.seq_slot[0]), place // 64])
+  for bad in (float("nan"), 3e38, -3e38, float("inf")):
+    spoiled = kv.clone()
+    spoiled[page, 0, :, place % 64, 3] = bad
+    out = torch.full_like(clean, 777.0)
+    ops.tree_attention(out, qkv, spoiled, *args[2:])
+    for t, s in enumerate(sees):
+      if not s:
+        assert torch.equal(out[t], clean[t])
+      elif bad != bad:
+        assert torch.isnan(out[t]).all()
+      else:
+        assert torch.isfinite(out[t]).all()
+
+
 def test_a_chain_is_causal_attention():
   """A tree without branches is a prompt portion: the same as ``attention`` gives."""
   from miniinfer_b200.kernels import ops
