@@ -516,7 +516,8 @@ class KVCacheManager:
       if src:
         lists = torch.tensor(src + dst + start, dtype=torch.int32).to(self.device)
         n = len(src)
-        ops.move_cache_rows(g.kv, lists[:n], lists[n:2 * n], lists[2 * n:], max(b - a for a, b in zip(start, start[1:])))
+        most = min(max(b - a for a, b in zip(start, start[1:])), 1024)      # (in order, so fewer at a time do too: no token moves back)
+        ops.move_cache_rows(g.kv, lists[:n], lists[n:2 * n], lists[2 * n:], most)
     for req_id, nodes in kept.items():
       rest = self._requests[req_id].reserved - len(nodes)
       self.commit(req_id, len(nodes))

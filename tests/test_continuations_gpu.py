@@ -171,3 +171,17 @@ def test_a_tree_of_which_a_path_is_accepted(dtype):
   out = attend(m, list(seqs), rows, [[1], [1]], [[len(seq)] for seq in seqs.values()])
   for o, seq in zip(out, seqs.values()):
     assert (o.double() - model.attention(seq + [7])).abs().max() < tol
+
+
+def test_more_tokens_are_kept_than_go_through_shared_memory_at_a_time():
+  m = KVCacheManager([PagedKVSpec(1, 16)], 64, 420, 2, 26000, torch.float32, DEV)
+  m.admit("a")
+  m.append("a", 26000)
+  places = torch.tensor(m.slot_mapping("a", 0, 0, 26000), device=DEV).long()
+  kv = m.paged_groups[0].kv
+  kv[0, places // 64, :, :, places % 64] = torch.arange(26000.0, device=DEV)[:, None, None, None]
+  m.keep({"a": list(range(1, 26000, 2))})
+  places = places[:13000]
+  assert m.length_of("a") == 13000
+  assert (kv[0, places // 64, :, :, places % 64] == torch.arange(1.0, 26000, 2, device=DEV)[:, None, None, None]).all()
+  m.check_invariants()
