@@ -16,8 +16,8 @@ namespace {
 
 using namespace mi_tree;
 
-// A warp has four rows.
-constexpr int threads_of(int rows) { return rows * 8; }
+// RG groups of four rows, KS warps a group.
+constexpr int threads_of(int RG, int KS) { return 32 * RG * KS; }
 
 template <typename T>
 __device__ __forceinline__ void load_row4(float4& v, const T* p, int left, bool wide) {      // four values, zeros past the row
@@ -34,11 +34,13 @@ __device__ __forceinline__ void load_row4(float4& v, const T* p, int left, bool 
 }
 
 // grid: (pieces, row tiles * nkv, items)
-template <typename T, int BR, int BK, int HD>
-__global__ void __launch_bounds__(threads_of(BR))
+template <typename T, int RG, int KS, int BK, int HD>
+__global__ void __launch_bounds__(threads_of(RG, KS))
 tree_kernel(Args a, int chunk, int pieces, int wide) {
-  constexpr int THREADS = threads_of(BR), TX = 32, KEYS = BK / TX, COLS = HD / (4 * TX);
-  static_assert(BK % TX == 0 && HD % (4 * TX) == 0, "a row's threads are a warp's");
+  constexpr int THREADS = threads_of(RG, KS), TX = 32, BR = 4 * RG, COLS = HD / (4 * TX);
+  constexpr int OWN = BK / KS;                              // keys of a tile that a warp has
+  constexpr int L = OWN < TX ? TX / OWN : 1, KEYS = OWN < TX ? 1 : OWN / TX;      // lanes that share a key's columns; keys of a lane
+  static_assert(BK % KS == 0 && OWN * L == TX * KEYS && L <= 4 && HD % (4 * TX) == 0, "a row's keys of a tile are a warp's lanes'");
   extern __shared__ __align__(16) float smem[];
   const int hd4 = (a.hd + 3) / 4, stride = 4 * hd4 + 4;      // a row in shared memory, 16 bytes on for the banks
   float *q_s = smem, *k_s = q_s + BR * stride, *v_s = k_s + BK * stride, *p_s = v_s + BK * stride;      // [BR, stride], [BK, stride] twice, [BR, BK + 4]
@@ -52,7 +54,9 @@ tree_kernel(Args a, int chunk, int pieces, int wide) {
   if (r0 >= rows) return;
   const int key_end = piece == pieces - 1 ? it.ctx : min(it.ctx, (piece + 1) * chunk);
   const int key_begin = max(piece * chunk, window_begin(a, it.start));      // (no new token's position is below the context's length)
-  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX % RG, split = threadIdx.x / TX / RG, own = split * OWN;
+  const int kx = tx % (TX / L), dx = tx / (TX / L);      // of the warp's keys; of the columns
+  const bool busy = r0 + 4 * ty < rows;      // one of the warp's rows exists; the other warps fetch only
   const T* qkv = reinterpret_cast<const T*>(a.qkv);
   const T* kv = reinterpret_cast<const T*>(a.kv);
 
@@ -114,56 +118,64 @@ tree_kernel(Args a, int chunk, int pieces, int wide) {
     if (more) find_rows(key0 + BK, buffer ^ 1);
     asm volatile("cp.async.wait_group 1;" ::: "memory");      // the keys are there
     __syncthreads();
-    float s[4][KEYS];
+    if (busy) {
+      float s[4][KEYS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < KEYS; ++j) s[i][j] = 0.f;
+        for (int j = 0; j < KEYS; ++j) s[i][j] = 0.f;
 #pragma unroll 2
-    for (int d = 0; d < 4 * hd4; d += 4) {
-      float4 q[4];
+      for (int d = 4 * dx; d < 4 * hd4; d += 4 * L) {
+        float4 q[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(q_s + (4 * ty + i) * stride + d);
+        for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(q_s + (4 * ty + i) * stride + d);
 #pragma unroll
-      for (int j = 0; j < KEYS; ++j) {
-        const float4 k = *reinterpret_cast<const float4*>(k_s + (tx + TX * j) * stride + d);
+        for (int j = 0; j < KEYS; ++j) {
+          const float4 k = *reinterpret_cast<const float4*>(k_s + (own + kx + TX * j) * stride + d);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i][j] = fmaf(q[i].w, k.w, fmaf(q[i].z, k.z, fmaf(q[i].y, k.y, fmaf(q[i].x, k.x, s[i][j]))));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float top = -INFINITY;
-      bool see[KEYS];
-#pragma unroll
-      for (int j = 0; j < KEYS; ++j) {
-        const int key = key0 + tx + TX * j, node = key - it.start;
-        see[j] = key < key_end;
-        if (node < 0) {
-          see[j] = see[j] && key >= begin[i];
-        } else if (see[j]) {
-          see[j] = (mask[i][node >> 5] >> (node & 31)) & 1;
-          if (a.window > 0) see[j] = see[j] && a.positions[it.row0 + node] >= begin[i];
+          for (int i = 0; i < 4; ++i) s[i][j] = fmaf(q[i].w, k.w, fmaf(q[i].z, k.z, fmaf(q[i].y, k.y, fmaf(q[i].x, k.x, s[i][j]))));
         }
-        s[i][j] = logit2_exact(s[i][j], a.scale, a.softcap);
-        if (see[j]) top = fmaxf(top, s[i][j]);
       }
 #pragma unroll
-      for (int o = TX / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float next = fmaxf(m[i], top), off = next == -INFINITY ? 0.f : next, alpha = exp2f(m[i] - off);
-      float part = 0.f;
+      for (int o = TX / L; o < TX; o <<= 1)
 #pragma unroll
-      for (int j = 0; j < KEYS; ++j) {
-        const float p = exp2f(s[i][j] - off);
-        if (see[j]) part += p;
-        p_s[(4 * ty + i) * PS + tx + TX * j] = see[j] ? p : -1.f;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < KEYS; ++j) s[i][j] += __shfl_xor_sync(0xffffffffu, s[i][j], o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float top = -INFINITY;
+        bool see[KEYS];
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j) {
+          const int key = key0 + own + kx + TX * j, node = key - it.start;
+          see[j] = key < key_end;
+          if (node < 0) {
+            see[j] = see[j] && key >= begin[i];
+          } else if (see[j]) {
+            see[j] = (mask[i][node >> 5] >> (node & 31)) & 1;
+            if (a.window > 0) see[j] = see[j] && a.positions[it.row0 + node] >= begin[i];
+          }
+          s[i][j] = logit2_exact(s[i][j], a.scale, a.softcap);
+          if (see[j]) top = fmaxf(top, s[i][j]);
+        }
+#pragma unroll
+        for (int o = TX / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float next = fmaxf(m[i], top), off = next == -INFINITY ? 0.f : next, alpha = exp2f(m[i] - off);
+        float part = 0.f;
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j) {
+          const float p = exp2f(s[i][j] - off);
+          if (see[j] && dx == 0) part += p;
+          if (dx == 0) p_s[(4 * ty + i) * PS + own + kx + TX * j] = see[j] ? p : -1.f;
+        }
+        m[i] = next;
+        l[i] = l[i] * alpha + part;      // (this thread's keys; the row's threads are added up at the end)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][c][e] *= alpha;
       }
-      m[i] = next;
-      l[i] = l[i] * alpha + part;      // (this thread's keys; the row's threads are added up at the end)
-#pragma unroll
-      for (int c = 0; c < COLS; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][c][e] *= alpha;
     }
     __syncthreads();      // (scores made, weights written)
     if (more) {
@@ -174,8 +186,8 @@ tree_kernel(Args a, int chunk, int pieces, int wide) {
     }
     __syncthreads();
     const bool all = key0 + BK <= min(it.start, key_end) && a.window <= 0;      // every row sees every key of the tile
-    const int near = min(BK, key_end - key0);
-    for (int k0 = 0; k0 < near; k0 += 4) {      // (past `near` all weights are -1)
+    const int near = busy ? min(own + OWN, key_end - key0) : 0;
+    for (int k0 = own; k0 < near; k0 += 4) {      // (past `near` all weights are -1)
       float4 p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(p_s + (4 * ty + i) * PS + k0);
@@ -205,11 +217,57 @@ tree_kernel(Args a, int chunk, int pieces, int wide) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int o = TX / 2; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+  if constexpr (KS > 1) {      // the row group's warps put together: warp `split` the rows split, split + KS, ..
+    float* acc_s = k_s;                                     // [KS, BR, stride], over the tiles
+    float2* ml_s = reinterpret_cast<float2*>(p_s);          // [KS, BR]
+    static_assert(KS * BR <= 2 * BK && 2 * KS <= PS, "the sums lie where the tiles were");
+    asm volatile("cp.async.wait_all;" ::: "memory");        // (those of a piece without keys)
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = split * BR + 4 * ty + i;
+      if (tx == 0) ml_s[at] = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+        if (4 * (tx + TX * c) < 4 * hd4) *reinterpret_cast<float4*>(acc_s + at * stride + 4 * (tx + TX * c)) = make_float4(acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i % KS != split) continue;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) top = fmaxf(top, ml_s[w * BR + 4 * ty + i].x);
+      const float off = top == -INFINITY ? 0.f : top;
+      m[i] = top;
+      l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) {
+        const int at = w * BR + 4 * ty + i;
+        const float2 x = ml_s[at];
+        const float weight = exp2f(x.x - off);
+        l[i] = fmaf(x.y, weight, l[i]);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+          if (4 * (tx + TX * c) < 4 * hd4) {
+            const float4 v = *reinterpret_cast<const float4*>(acc_s + at * stride + 4 * (tx + TX * c));
+            acc[i][c][0] = fmaf(v.x, weight, acc[i][c][0]);
+            acc[i][c][1] = fmaf(v.y, weight, acc[i][c][1]);
+            acc[i][c][2] = fmaf(v.z, weight, acc[i][c][2]);
+            acc[i][c][3] = fmaf(v.w, weight, acc[i][c][3]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     const int row = r0 + 4 * ty + i;
-    if (row >= rows) continue;
+    if (row >= rows || i % KS != split) continue;
     const int h = head * a.G + row % a.G;
     const size_t at = (size_t)(it.row0 + token[i]) * a.nh + h;
     if (pieces > 1) {
@@ -285,8 +343,9 @@ tree_merge_kernel(Args a, int chunk, int pieces) {
   }
 }
 
-template <typename T, int BR, int BK, int HD>
+template <typename T, int RG, int KS, int BK, int HD>
 int launch(const Args& a, int chunk, int pieces, bool wide, cudaStream_t stream) {
+  constexpr int BR = 4 * RG;
   const int stride = (a.hd + 3) / 4 * 4 + 4;
   const size_t smem = ((size_t)(BR + 2 * BK) * stride + BR * (BK + 4)) * sizeof(float);
   static bool ready[64] = {};
@@ -294,18 +353,34 @@ int launch(const Args& a, int chunk, int pieces, bool wide, cudaStream_t stream)
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return mi_fail("attention_tree: no current device");
   if (!ready[dev]) {
     const size_t most = ((size_t)(BR + 2 * BK) * (HD + 4) + BR * (BK + 4)) * sizeof(float);
-    if (cudaFuncSetAttribute(tree_kernel<T, BR, BK, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
+    if (cudaFuncSetAttribute(tree_kernel<T, RG, KS, BK, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
       return mi_fail("attention_tree: %zu bytes of shared memory were refused", most);
     ready[dev] = true;
   }
   const int tiles = (a.max_q * a.G + BR - 1) / BR;
   MI_REQUIRE((long long)tiles * a.nkv <= 65535, "attention_tree: %d rows of %d heads are too many for one launch", a.max_q * a.G, a.nkv);
-  if (mi::launch(tree_kernel<T, BR, BK, HD>, dim3(pieces, tiles * a.nkv, a.items), dim3(threads_of(BR)), smem, stream, a, chunk, pieces, (int)wide) != cudaSuccess)
+  if (mi::launch(tree_kernel<T, RG, KS, BK, HD>, dim3(pieces, tiles * a.nkv, a.items), dim3(threads_of(RG, KS)), smem, stream, a, chunk, pieces, (int)wide) != cudaSuccess)
     return mi_fail("attention_tree: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   if (pieces > 1 && mi::launch(tree_merge_kernel<T>, dim3(a.T, (a.nh + 3) / 4), dim3(128), 0, stream, a, chunk, pieces) != cudaSuccess)
     return mi_fail("attention_tree: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   MI_LAUNCH_OK("attention_tree");
   return 0;
+}
+
+// All eight warps have a row group each, or with few rows several of them share a group's keys.
+template <typename T, int HD>
+int launch_rows(const Args& a, int chunk, int pieces, bool wide, cudaStream_t stream) {
+  const int rows = a.max_q * a.G;
+  if (rows <= 4) return launch<T, 1, 8, 64, HD>(a, chunk, pieces, wide, stream);
+  if (rows <= 8) return launch<T, 2, 4, 64, HD>(a, chunk, pieces, wide, stream);
+  if (rows <= 16) return launch<T, 4, 2, 64, HD>(a, chunk, pieces, wide, stream);
+  return launch<T, 8, 1, 64, HD>(a, chunk, pieces, wide, stream);
+}
+template <typename T>
+int launch_sized(const Args& a, int chunk, int pieces, bool wide, cudaStream_t stream) {
+  if (a.hd <= 128) return launch_rows<T, 128>(a, chunk, pieces, wide, stream);
+  if (a.hd <= 256) return launch_rows<T, 256>(a, chunk, pieces, wide, stream);
+  return launch<T, 4, 1, 32, 640>(a, chunk, pieces, wide, stream);
 }
 
 }  // namespace
@@ -326,10 +401,6 @@ MI_API int mi_attention_tree(void* out, const void* qkv, int dtype, const void* 
   const int size = dtype == MI_F32 ? 4 : 2;
   const bool wide = hd % 4 == 0 && (long long)width % 4 == 0 && (((uintptr_t)qkv | (uintptr_t)kv) % (4 * size)) == 0;
   MI_REQUIRE(dtype == MI_F32 || dtype == MI_BF16, "attention_tree: unknown type");
-  if (dtype == MI_F32) {
-    if (hd <= 128) return launch<float, 32, 64, 128>(a, chunk, pieces, wide, stream);
-    return hd <= 256 ? launch<float, 32, 64, 256>(a, chunk, pieces, wide, stream) : launch<float, 16, 32, 640>(a, chunk, pieces, wide, stream);
-  }
-  if (hd <= 128) return launch<__nv_bfloat16, 32, 64, 128>(a, chunk, pieces, wide, stream);
-  return hd <= 256 ? launch<__nv_bfloat16, 32, 64, 256>(a, chunk, pieces, wide, stream) : launch<__nv_bfloat16, 16, 32, 640>(a, chunk, pieces, wide, stream);
+  if (dtype == MI_F32) return launch_sized<float>(a, chunk, pieces, wide, stream);
+  return launch_sized<__nv_bfloat16>(a, chunk, pieces, wide, stream);
 }

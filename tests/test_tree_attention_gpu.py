@@ -52,6 +52,16 @@ def test_tree_attention(case, dtype):
   assert close_enough(out, terms, dtype, args[6], int(args[3].max_ctx_len), args[10]) <= 1.0
 
 
+@pytest.mark.parametrize("hd,page", [(128, 64), (256, 64), (100, 7)])
+@pytest.mark.parametrize("rows", [1, 3, 4, 5, 8, 9, 16, 17])
+def test_few_rows_in_32_bits(rows, hd, page):
+  """Up to 16 rows several warps share a row's keys: contexts that end in each warp's share of a tile, and rows that see few of them."""
+  group = 1 if rows % 2 else 2
+  items = [(c, rows // group) for c in (0, 5, 30, 61, 64, 700, 1333)]
+  out, args = run((items, 2 * group, 2, hd, page, 90, rows % 3 == 0, 0.0, 0.2), torch.float32)
+  assert close_enough(out, torch_ops.tree_terms(*args), torch.float32, hd, 1400) <= 1.0
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_between_requests_are_left_and_slack_in_the_sizes_does_not_matter(dtype):
   from miniinfer_b200.engine.context import Workspace
