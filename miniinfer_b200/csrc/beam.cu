@@ -388,13 +388,16 @@ beam_select_kernel(Args a) {
   constexpr int PER = 16 / sizeof(T);
   const uint32_t my_stage = (uint32_t)__cvta_generic_to_shared(stages) + threadIdx.x * 16;
   const int mine0 = first + (int)threadIdx.x * PER;      // the thread's first value of the first tile
-  if constexpr (WIDE) {
+  auto fetch_first = [&]() {
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) {
-      fetch<T>(my_stage + t * STAGE_BYTES, x + mine0 + t * TILE, end - mine0 - t * TILE);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      for (int t = 0; t < STAGES - 1; ++t) {
+        fetch<T>(my_stage + t * STAGE_BYTES, x + mine0 + t * TILE, end - mine0 - t * TILE);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
     }
-  }
+  };
+  fetch_first();
   if (warp == 0) {
     const int q = request_of(a, row);
     if (lane == 0) {
@@ -411,98 +414,114 @@ beam_select_kernel(Args a) {
     const float b = keep_best(pool, &s_count, a.n, lists);
     if (b > bar) bar = b;
   };
+  // Warps collect what beats the bar as it comes, each at its own pace; they meet where the bar rises.  Should there be no room for all (a row whose tiles get
+  // better and better), the stretch is walked once more, all threads' candidates of a tile counted before they are collected.
 #pragma unroll 1
-  for (int t = 0; t < tiles; ++t) {
-    const int begin = first + t * TILE;
-    if constexpr (WIDE) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-    float v[ITEMS];
-    read_tile<T, WIDE>(v, stages + t % STAGES * STAGE_BYTES, x, begin, end);
-    if constexpr (WIDE) {      // into the stage that was read a tile ago
-      const int ahead = (t + STAGES - 1) * TILE;
-      fetch<T>(my_stage + (t + STAGES - 1) % STAGES * STAGE_BYTES, x + mine0 + ahead, end - mine0 - ahead);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    float top = v[0];
-#pragma unroll
-    for (int j = 1; j < ITEMS - 1; j += 2) top = mi::max_of(top, v[j], v[j + 1]);
-    top = fmaxf(top, v[ITEMS - 1]);
-    if (top > m) {
-      sum *= mi::ex2_fast((m - top) * 1.4426950408889634f);
-      m = top;
-    }
-    const float off = m == -INFINITY ? 0.f : -m;
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < ITEMS; j += 2) {      // (the difference first: values may be as large as they get)
-      float d0 = v[j], d1 = v[j + 1];
-      mi::add_pair(d0, d1, off, off);
-      mi::mul_pair(d0, d1, d0, d1, 1.4426950408889634f);
-      mi::add_pair(part[j & 2], part[(j & 2) + 1], mi::ex2_fast(d0), mi::ex2_fast(d1));
-    }
-    sum += (part[0] + part[1]) + (part[2] + part[3]);
-    // who has a value that beats the bar; `most`: the candidates that may be there by now, counted without asking (a barrier less)
-    int beating = __syncthreads_count(top > bar);
-    if (beating == 0) continue;
-    if (most + beating * ITEMS > ROOM && most > a.n) {
-      thin_out();
-      most = a.n;
-      beating = __syncthreads_count(top > bar);
-    }
-    uint32_t hits = 0;
-    if (top > bar) {
-#pragma unroll
-      for (int j = 0; j < ITEMS; ++j) hits |= (v[j] > bar ? 1u : 0u) << j;
-    }
-    // (values by their number out of the stage or the row: registers cannot be asked by number)
-    auto key_by_number = [&](int j) {
-      const int token = token_at<T, WIDE>(begin, j);
-      if constexpr (WIDE) {
-        return key_of(mi::to_float(reinterpret_cast<const T*>(stages + t % STAGES * STAGE_BYTES)[(j / PER * THREADS + (int)threadIdx.x) * PER + j % PER]), token);
-      } else {
-        return key_of(mi::to_float(x[token]), token);
+  for (bool counted = false;; counted = true) {
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      const int begin = first + t * TILE;
+      if constexpr (WIDE) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      float v[ITEMS];
+      read_tile<T, WIDE>(v, stages + t % STAGES * STAGE_BYTES, x, begin, end);
+      if constexpr (WIDE) {      // into the stage that was read a tile ago
+        const int ahead = (t + STAGES - 1) * TILE;
+        fetch<T>(my_stage + (t + STAGES - 1) % STAGES * STAGE_BYTES, x + mine0 + ahead, end - mine0 - ahead);
+        asm volatile("cp.async.commit_group;" ::: "memory");
       }
-    };
-    const bool bounded = t == 0 || most + beating * ITEMS > ROOM;      // (the first tile has no bar: all of a small vocabulary would be ranked)
-    if (bounded) {
-      const int before = s_count;
-      const uint32_t high = top > -INFINITY ? rising(top) : 0;
-      uint64_t bound = (uint64_t)quick_bound(high, a.n, of_warp) << 32;
-#pragma unroll 1
-      for (bool again = false;; again = true) {
-        const float least = bound ? value_of(bound) : -INFINITY;
-        uint32_t mine = 0;
+      float top = v[0];
 #pragma unroll
-        for (int j = 0; j < ITEMS; ++j) mine |= (v[j] >= least ? 1u : 0u) << j;
-        mine &= hits;
-#pragma unroll 1
-        for (uint32_t todo = mine; todo; todo &= todo - 1)      // (of equal values the lower tokens)
-          if (key_by_number(__ffs(todo) - 1) < bound) mine &= ~(todo & -todo);
-        int i = mine ? atomicAdd(&s_count, __popc(mine)) : 0;
-#pragma unroll 1
-        for (; mine && i < ROOM; mine &= mine - 1) pool[i++] = key_by_number(__ffs(mine) - 1);
-        __syncthreads();
-        if (again || s_count - before <= MANY) break;
-        uint64_t best = 0;      // more than are ranked in a moment: the exact bound of the threads' bests
-#pragma unroll
-        for (int j = ITEMS - 1; j >= 0; --j)
-          if (v[j] == top && top > bar) best = key_of(top, token_at<T, WIDE>(begin, j));
-        bound = nth_best(best, a.n, lists, &s_nth);
-        if (threadIdx.x == 0) s_count = before;
-        __syncthreads();
+      for (int j = 1; j < ITEMS - 1; j += 2) top = mi::max_of(top, v[j], v[j + 1]);
+      top = fmaxf(top, v[ITEMS - 1]);
+      if (top > m) {
+        sum *= mi::ex2_fast((m - top) * 1.4426950408889634f);
+        m = top;
       }
-    } else if (hits) {
-      int i = atomicAdd(&s_count, __popc(hits));
+      const float off = m == -INFINITY ? 0.f : -m;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < ITEMS; j += 2) {      // (the difference first: values may be as large as they get)
+        float d0 = v[j], d1 = v[j + 1];
+        mi::add_pair(d0, d1, off, off);
+        mi::mul_pair(d0, d1, d0, d1, 1.4426950408889634f);
+        mi::add_pair(part[j & 2], part[(j & 2) + 1], mi::ex2_fast(d0), mi::ex2_fast(d1));
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      int beating = 0;
+      if (counted || t == 0) {
+        // who has a value that beats the bar; `most`: the candidates that may be there by now, counted without asking (a barrier less)
+        beating = __syncthreads_count(top > bar);
+        if (beating == 0) continue;
+        if (most + beating * ITEMS > ROOM && most > a.n) {
+          thin_out();
+          most = a.n;
+          beating = __syncthreads_count(top > bar);
+        }
+      }
+      uint32_t hits = 0;
+      if (top > bar) {
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) hits |= (v[j] > bar ? 1u : 0u) << j;
+      }
+      // (values by their number out of the stage or the row: registers cannot be asked by number)
+      auto key_by_number = [&](int j) {
+        const int token = token_at<T, WIDE>(begin, j);
+        if constexpr (WIDE) {
+          return key_of(mi::to_float(reinterpret_cast<const T*>(stages + t % STAGES * STAGE_BYTES)[(j / PER * THREADS + (int)threadIdx.x) * PER + j % PER]), token);
+        } else {
+          return key_of(mi::to_float(x[token]), token);
+        }
+      };
+      const bool bounded = t == 0 || (counted && most + beating * ITEMS > ROOM);      // (the first tile has no bar: all of a small vocabulary would be ranked)
+      if (bounded) {
+        const int before = s_count;
+        const uint32_t high = top > -INFINITY ? rising(top) : 0;
+        uint64_t bound = (uint64_t)quick_bound(high, a.n, of_warp) << 32;
 #pragma unroll 1
-      for (; hits; hits &= hits - 1) pool[i++] = key_by_number(__ffs(hits) - 1);
+        for (bool again = false;; again = true) {
+          const float least = bound ? value_of(bound) : -INFINITY;
+          uint32_t mine = 0;
+#pragma unroll
+          for (int j = 0; j < ITEMS; ++j) mine |= (v[j] >= least ? 1u : 0u) << j;
+          mine &= hits;
+#pragma unroll 1
+          for (uint32_t todo = mine; todo; todo &= todo - 1)      // (of equal values the lower tokens)
+            if (key_by_number(__ffs(todo) - 1) < bound) mine &= ~(todo & -todo);
+          int i = mine ? atomicAdd(&s_count, __popc(mine)) : 0;
+#pragma unroll 1
+          for (; mine && i < ROOM; mine &= mine - 1) pool[i++] = key_by_number(__ffs(mine) - 1);
+          __syncthreads();
+          if (again || s_count - before <= MANY) break;
+          uint64_t best = 0;      // more than are ranked in a moment: the exact bound of the threads' bests
+#pragma unroll
+          for (int j = ITEMS - 1; j >= 0; --j)
+            if (v[j] == top && top > bar) best = key_of(top, token_at<T, WIDE>(begin, j));
+          bound = nth_best(best, a.n, lists, &s_nth);
+          if (threadIdx.x == 0) s_count = before;
+          __syncthreads();
+        }
+      } else if (hits) {
+        int i = atomicAdd(&s_count, __popc(hits));
+#pragma unroll 1
+        for (; hits && i < ROOM; hits &= hits - 1) pool[i++] = key_by_number(__ffs(hits) - 1);
+      }
+      most = bounded ? ROOM : most + beating * ITEMS;
+      if (t == 0 || t == 3 || t == 15) {      // the bar rises as the tiles say less
+        __syncthreads();
+        if (s_count > ROOM) break;
+        thin_out();
+        most = a.n;
+      }
     }
-    most = bounded ? ROOM : most + beating * ITEMS;
-    if (t == 0 || t == 3 || t == 15) {      // the bar rises as the tiles say less
-      __syncthreads();
-      thin_out();
-      most = a.n;
-    }
+    __syncthreads();
+    if (counted || s_count <= ROOM) break;
+    __syncthreads();
+    if (threadIdx.x == 0) s_count = 0;
+    m = bar = -INFINITY;
+    sum = 0.f;
+    if constexpr (WIDE) asm volatile("cp.async.wait_all;" ::: "memory");
+    fetch_first();
   }
-  __syncthreads();
   thin_out();
   const int got = s_count;
   uint64_t* best = a.best + ((size_t)row * a.stretches + stretch) * a.n;

@@ -179,3 +179,18 @@ def test_rows_of_no_request_and_lists_that_end_behind_the_rows(start):
   cut = [min(s, 5) for s in start]
   for _ in range(2):      # (the second call finds the counters as the first left them)
     check(select(logits, cum, start, 7), logits, cum, cut, 7)
+
+
+@pytest.mark.parametrize("V", [50000, 50001])
+@pytest.mark.parametrize("n", [3, 128])
+def test_many_rows_whose_best_come_early_or_late(n, V):
+  """A block walks a whole row: rising rows have more candidates than there is room for, others none in their first tiles, or no more than n."""
+  at = torch.arange(V).float()
+  rows = [at * 1e-4, -at * 1e-4, (at - 30000).abs() * 1e-4, torch.where(at < 20000, NINF, at * 1e-4), torch.where(at < 4096, NINF, -at * 1e-4),
+          torch.where(at % 997 == 5, at * 1e-3, NINF), torch.zeros(V), torch.floor(at / 8192), torch.floor(at / 700), torch.where(at == V - 1, 1.0, NINF),
+          torch.full((V,), NINF), torch.randn(V, generator=torch.Generator().manual_seed(V))]
+  logits = torch.stack(rows * 13).to(DEV)
+  cum = torch.randn(len(logits), generator=torch.Generator().manual_seed(n)).to(DEV)
+  cum = cum + torch.arange(len(logits), device=DEV) * 10      # (so that rows do not tie)
+  for start in (list(range(len(logits) + 1)), [0, 12, 24, 36, len(logits)]):
+    check(select(logits, cum, start, n), logits, cum, start, n)
