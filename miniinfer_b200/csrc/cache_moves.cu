@@ -11,6 +11,10 @@
 //
 // Nothing is computed; the bytes are the bound.  Loads are asynchronous copies of 16 bytes into shared memory (of 4 or 2 where rows
 // or the base are not aligned to more), so what a block has on its way is its whole share and not its registers.
+//
+// Measured: 96 pages of 28 layers (1.41 GB read and written) 216 us, 6.5 TB/s, the rate of a plain copy; paths of 8 of 64 tokens for 64 requests (117 MB)
+// 20.5 us, 5.7 TB/s; 32 states of 12 layers of 1 MB 81 us (what keeps its place costs nothing); 3 pages (15 MB) 7.6 us; calls of a MB or less 1.9 to 2.5 us,
+// which a launch takes.
 #include "common.cuh"
 
 namespace {
