@@ -13,7 +13,7 @@
 // or the base are not aligned to more), so what a block has on its way is its whole share and not its registers.
 //
 // Measured: 96 pages of 28 layers (1.41 GB read and written) 216 us, 6.5 TB/s, the rate of a plain copy; paths of 8 of 64 tokens for 64 requests (117 MB)
-// 20.5 us, 5.7 TB/s; 32 states of 12 layers of 1 MB 81 us (what keeps its place costs nothing); 3 pages (15 MB) 7.6 us; calls of a MB or less 1.9 to 2.5 us,
+// 20.5 us, 5.7 TB/s; 32 states of 12 layers of 1 MB 81 us (what keeps its place costs nothing); 3 pages (15 MB) 6.9 us; calls of a MB or less 1.9 to 2.5 us,
 // which a launch takes.
 #include "common.cuh"
 
@@ -48,20 +48,19 @@ struct Places {
 };
 
 // One block: a few columns of layer blockIdx.y, of all pairs.  A thread stays in its column; 2^log_columns threads side by side take a pair.
-template <typename U, bool FILLED>
+template <typename U>
 __global__ void __launch_bounds__(THREADS) move_places_kernel(Places a) {
   extern __shared__ __align__(16) unsigned char smem[];
   U* stage = reinterpret_cast<U*>(smem);                                                     // [n, columns]
   const int columns = 1 << a.log_columns, c = threadIdx.x & (columns - 1), k0 = threadIdx.x >> a.log_columns, step = THREADS >> a.log_columns;
   const long long at = ((long long)blockIdx.x << a.log_columns) + c;
   U* column = reinterpret_cast<U*>(a.base) + (long long)blockIdx.y * a.places * a.row_units + at;
-  const int row = FILLED ? (int)(at / a.token_units % a.page) : 0;
   mi::grid_dependency_sync();
   if (at < a.row_units) {
 #pragma unroll 4
     for (int k = k0; k < a.n; k += step) {
       const int from = a.src[k], to = a.dst[k];
-      const bool wanted = (unsigned)from < (unsigned long long)a.places && (unsigned)to < (unsigned long long)a.places && from != to && (!FILLED || row < a.filled[k]);
+      const bool wanted = (unsigned)from < (unsigned long long)a.places && (unsigned)to < (unsigned long long)a.places && from != to;
       if (wanted) copy_to_shared(stage + (k << a.log_columns) + c, column + from * a.row_units);
     }
   }
@@ -70,10 +69,46 @@ __global__ void __launch_bounds__(THREADS) move_places_kernel(Places a) {
 #pragma unroll 4
     for (int k = k0; k < a.n; k += step) {
       const int from = a.src[k], to = a.dst[k];
-      const bool wanted = (unsigned)from < (unsigned long long)a.places && (unsigned)to < (unsigned long long)a.places && from != to && (!FILLED || row < a.filled[k]);
+      const bool wanted = (unsigned)from < (unsigned long long)a.places && (unsigned)to < (unsigned long long)a.places && from != to;
       if (wanted) column[to * a.row_units] = stage[(k << a.log_columns) + c];
     }
   }
+}
+
+// The same for places that are filled in part: a block lists the pairs that have something in its columns first, for half of them as a rule have not
+// (465 pairs of pages filled to any length, 20 layers, 152 MB: 32 us instead of 67; 3 pairs of 28 layers 6.9 instead of 7.6).
+template <typename U>
+__global__ void __launch_bounds__(THREADS) move_filled_kernel(Places a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  int* list = reinterpret_cast<int*>(smem);                                                  // [3][n]: from, to, filled
+  U* stage = reinterpret_cast<U*>(smem + (a.n * 12 + 15) / 16 * 16);                         // [n, columns]
+  __shared__ int count;
+  const unsigned columns = 1u << a.log_columns, c = threadIdx.x & (columns - 1), first = blockIdx.x << a.log_columns, at = first + c;
+  const int k0 = threadIdx.x >> a.log_columns, step = THREADS >> a.log_columns;
+  const unsigned token_first = first / a.token_units, token_last = (min(first + columns, (unsigned)a.row_units) - 1) / a.token_units, token = at / a.token_units;
+  const int row = token % a.page, lowest = token_first / a.page == token_last / a.page ? token_first % a.page : 0;      // of the thread's column; of the block's
+  U* column = reinterpret_cast<U*>(a.base) + (long long)blockIdx.y * a.places * a.row_units + at;
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  mi::grid_dependency_sync();
+  for (int k = threadIdx.x; k < a.n; k += THREADS) {
+    const int from = a.src[k], to = a.dst[k], filled = a.filled[k];
+    if ((unsigned)from < (unsigned long long)a.places && (unsigned)to < (unsigned long long)a.places && from != to && lowest < filled) {
+      const int i = atomicAdd(&count, 1);      // (in any order: destinations differ)
+      list[i] = from;
+      list[a.n + i] = to;
+      list[2 * a.n + i] = filled;
+    }
+  }
+  __syncthreads();
+  const int n = at < a.row_units ? count : 0;
+#pragma unroll 4
+  for (int k = k0; k < n; k += step)
+    if (row < list[2 * a.n + k]) copy_to_shared(stage + (k << a.log_columns) + c, column + list[k] * a.row_units);
+  copies_done();
+#pragma unroll 4
+  for (int k = k0; k < n; k += step)
+    if (row < list[2 * a.n + k]) column[list[a.n + k] * a.row_units] = stage[(k << a.log_columns) + c];
 }
 
 struct Rows {
@@ -153,19 +188,20 @@ int allow_shared(K kernel, bool* ready) {      // more shared memory than a kern
 template <typename U, bool FILLED>
 int launch_places(Places a, int layers, cudaStream_t stream) {
   static bool ready[64] = {};
-  if (allow_shared(move_places_kernel<U, FILLED>, ready)) return 1;
+  auto kernel = FILLED ? move_filled_kernel<U> : move_places_kernel<U>;
+  if (allow_shared(kernel, ready)) return 1;
   // columns: what the wanted shared memory holds, at least 8 (128 bytes in a row) as long as the most allows, no more than a place or the threads have,
   // and few enough that small calls are spread over the GPU
-  const long long per = (long long)a.n * sizeof(U), spread = (a.row_units * layers + 4 * mi::sm_count() - 1) / (4 * mi::sm_count());
+  const long long list = FILLED ? (a.n * 12ll + 15) / 16 * 16 : 0, per = (long long)a.n * sizeof(U), spread = (a.row_units * layers + 4 * mi::sm_count() - 1) / (4 * mi::sm_count());
   long long most = SMEM_WANTED / per;
   if (most < 8) most = 8;
-  if (most > SMEM_MOST / per) most = SMEM_MOST / per;
+  if (most > (SMEM_MOST - list) / per) most = (SMEM_MOST - list) / per;
   if (most > (spread > 16 ? spread : 16)) most = spread > 16 ? spread : 16;
   a.log_columns = 0;
   while ((2ll << a.log_columns) <= most && (2 << a.log_columns) <= THREADS && (1ll << a.log_columns) < a.row_units) ++a.log_columns;
   const long long c = 1ll << a.log_columns, blocks = (a.row_units + c - 1) / c;
   MI_REQUIRE(blocks <= 0x7fffffffll && layers <= 65535, "cache moves: %lld blocks of %d layers are too many for one launch", blocks, layers);
-  if (mi::launch(move_places_kernel<U, FILLED>, dim3((unsigned)blocks, layers), dim3(THREADS), (size_t)(per * c), stream, a) != cudaSuccess)
+  if (mi::launch(kernel, dim3((unsigned)blocks, layers), dim3(THREADS), (size_t)(list + per * c), stream, a) != cudaSuccess)
     return mi_fail("cache moves: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   MI_LAUNCH_OK("cache moves");
   return 0;
@@ -203,6 +239,7 @@ MI_API int mi_move_places(void* base, int layers, long long places, long long pl
   if (layers == 0 || places == 0 || place_bytes == 0 || n == 0) return 0;
   MI_REQUIRE(places <= 0x7fffffffll, "cache moves: %lld places are too many", places);
   if (filled) MI_REQUIRE(page > 0 && token_bytes > 0 && place_bytes % (page * token_bytes) == 0, "cache moves: a place of %lld bytes is not made of %d rows of %lld", place_bytes, page, token_bytes);
+  if (filled) MI_REQUIRE(place_bytes <= 0x7fffffffll, "cache moves: a place of %lld bytes is too large to be copied in part", place_bytes);
   const int unit = unit_of(base, filled ? (place_bytes | token_bytes) : place_bytes);
   Places a{base, src, dst, filled, places, place_bytes / unit, n, 0, page, filled ? (int)(token_bytes / unit) : 1};
   if (filled) {

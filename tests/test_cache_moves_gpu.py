@@ -147,3 +147,16 @@ def test_captured_and_replayed():
     torch_ops.move_cache_rows(want_kv, src, dst, start, 2)
     graph.replay()
     assert torch.equal(state, want_state) and torch.equal(kv, want_kv)
+
+
+@pytest.mark.parametrize("heads,P,hd,pairs", [(1, 4, 16, 4096), (3, 7, 5, 1000), (2, 64, 64, 300), (1, 1, 8, 40)])
+def test_many_pages_in_part(heads, P, hd, pairs):
+  """Lists of up to the most pairs, of pages that are filled to any length, not at all, beyond their end, or padded."""
+  rng = random.Random(pairs)
+  ids = list(range(2 * pairs + 1))
+  rng.shuffle(ids)
+  src, dst = ids[:pairs], ids[pairs:2 * pairs]
+  dst[1], src[2], src[3], dst[4] = -1, len(ids), dst[5], src[5]      # padding, out of range, a page that is written and read, and one read and written
+  filled = [rng.randint(-1, P + 1) for _ in src]
+  kv = filled_tensor((2, len(ids), 2, heads, P, hd), torch.bfloat16, P)
+  compare("copy_cache_pages", kv, ints(src), ints(dst), ints(filled))
