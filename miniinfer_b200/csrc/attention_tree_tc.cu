@@ -665,7 +665,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       const int hidden_from = p.it.start, hidden_to = a.window > 0 ? p.it.start + p.it.n - a.window : 0;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = KEYS ? set : 0; j < tiles; j += KEYS ? 2 : 1, ++g) {
-        const bool first_of_set = j < SETS;
+        const bool first_of_set = j < (KEYS ? 2 : 1);      // of this piece's tiles; two sets of rows both begin with tile 0
         const int key0 = p.key + j * BN;
         const bool masked = key0 + BN > hidden_from || key0 < hidden_to;
         uint32_t bits[BN / 32];      // keys that the row sees
