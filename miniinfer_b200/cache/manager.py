@@ -430,18 +430,19 @@ class KVCacheManager:
     return new
 
   def _copy_on_device(self, copies: List[List[tuple]], slots: List[tuple]) -> None:
-    """The pages' copies, a launch a group, and those of the states of ``slots`` - (from, to)."""
+    """The pages' copies, a launch a group, and those of the states of ``slots`` - (from, to) -, as many in a launch as one takes: no place is
+    both copied from and to, so their order does not matter."""
     def lists(rows):
-      return torch.tensor(rows, dtype=torch.int32).t().contiguous().to(self.device)
+      for i in range(0, len(rows), ops.MOVE_MAX_PAIRS):
+        yield torch.tensor(rows[i:i + ops.MOVE_MAX_PAIRS], dtype=torch.int32).t().contiguous().to(self.device)
 
     for g, todo in zip(self.paged_groups, copies):
-      for i in range(0, len(todo), ops.MOVE_MAX_PAIRS):
-        src, dst, filled = lists(todo[i:i + ops.MOVE_MAX_PAIRS])
+      for src, dst, filled in lists(todo):
         ops.copy_cache_pages(g.kv, src, dst, filled)
-    if slots:
-      src, dst = lists(slots)
-      for s in self.state_groups:
-        ops.reorder_states(s.state, src, dst)
+    if self.state_groups:
+      for src, dst in lists(slots):
+        for s in self.state_groups:
+          ops.reorder_states(s.state, src, dst)
 
   def fork(self, req_id: Hashable, children: Sequence[Hashable]) -> None:
     """Admits ``children``, each of which goes on from where the request is, its states with it: full pages are shared, what the last, partly

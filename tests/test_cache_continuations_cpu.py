@@ -181,3 +181,31 @@ def test_a_composite_layer_is_forked_whole():
   m.commit("a", 3)
   m.fork("a", ["b"])
   check(m, {"a": [1, 2, 3], "b": [1, 2, 3]})
+
+
+def test_more_copies_than_go_in_one_call(monkeypatch):
+  """A call of the copies takes MOVE_MAX_PAIRS pairs at most, of pages and of states."""
+  from miniinfer_b200.kernels import ops
+  most, calls = 3, []
+  monkeypatch.setattr(ops, "MOVE_MAX_PAIRS", most)
+  for name in ("copy_cache_pages", "reorder_states"):
+    def limited(base, src, *rest, plain=getattr(ops, name), name=name):
+      if src.shape[0] > most:
+        raise ops.KernelError(f"{src.shape[0]} pairs")
+      calls.append((name, src.shape[0]))
+      plain(base, src, *rest)
+    monkeypatch.setattr(ops, name, limited)
+  m = make(seqs=9, state=True)
+  m.admit(0)
+  write(m, 0, [1, 2, 3, 4, 5])
+  m.commit(0, 5)
+  m.fork(0, range(1, 9))
+  seqs = {q: [1, 2, 3, 4, 5] for q in range(9)}
+  check(m, seqs)
+  assert sorted(calls) == sorted([("copy_cache_pages", n) for n in (3, 3, 2)] + [("reorder_states", n) for n in (3, 3, 2)])
+  for q in range(9):
+    write(m, q, [10 + q])
+    m.commit(q, 1)
+    seqs[q] = seqs[q] + [10 + q]
+  m.reorder({q: 4 + q % 2 for q in range(9)})
+  check(m, {q: seqs[4 + q % 2] for q in range(9)})
