@@ -414,17 +414,15 @@ class KVCacheManager:
       raise ValueError(f"request {req_id!r} has {r.reserved} tokens that are neither committed nor cancelled")
     return r
 
-  def _copy_of(self, r: _Request, slot: int, copies: List[List[tuple]]) -> _Request:
-    """A request in ``slot`` that goes on from where ``r`` is: its full pages shared, a page of its own for what a last page holds.  The pages to
-    copy - (from, to, tokens) - are put into ``copies``, a list a group; the caller has seen to it that there are pages."""
+  def _copy_of(self, r: _Request, slot: int, fresh: List[Optional[int]]) -> _Request:
+    """A request in ``slot`` that goes on from where ``r`` is: its full pages shared, and where the last one holds something ``fresh`` - a page a
+    group, held already - in its place."""
     new = _Request(slot=slot, length=r.length, pages=[list(p) for p in r.pages])
-    for g, todo in zip(self.paged_groups, copies):
-      mine, filled = new.pages[g.index], r.length % g.page_size
-      if filled:
-        page = g.allocator.alloc(1)[0]
-        todo.append((mine[-1], page, filled))
+    for g, page in zip(self.paged_groups, fresh):
+      mine = new.pages[g.index]
+      g.allocator.share([p for p in (mine if page is None else mine[:-1]) if p])
+      if page is not None:
         mine[-1] = page
-      g.allocator.share([p for p in (mine[:-1] if filled else mine) if p])
       g.block_table_host[slot, :len(mine)] = mine
       g._dirty.add(slot)
     return new
@@ -446,7 +444,7 @@ class KVCacheManager:
 
   def fork(self, req_id: Hashable, children: Sequence[Hashable]) -> None:
     """Admits ``children``, each of which goes on from where the request is, its states with it: full pages are shared, what the last, partly
-    filled page holds is copied.  ``OutOfSlots`` or ``OutOfPages`` change nothing."""
+    filled page holds is copied.  ``OutOfSlots``, ``OutOfPages`` or an error of the copies' launches change nothing."""
     r, n = self._settled(req_id), len(children)
     if len(set(children)) < n or any(c in self._requests for c in children):
       raise KeyError("a child is already admitted, or named twice")
@@ -455,18 +453,23 @@ class KVCacheManager:
     for g in self.paged_groups:
       if r.length % g.page_size and n > g.allocator.num_free:
         raise OutOfPages(f"group {g.index}: {n} pages wanted for copies of request {req_id!r}, {g.allocator.num_free} of {g.num_pages} free")
-    copies: List[List[tuple]] = [[] for _ in self.paged_groups]
-    slots = []
-    for c in children:
-      slot = self._free_slots.pop()
-      self._requests[c] = self._copy_of(r, slot, copies)
-      slots.append((r.slot, slot))
-    self._copy_on_device(copies, slots)
+    fresh = [g.allocator.alloc(n) if r.length % g.page_size else [None] * n for g in self.paged_groups]
+    slots = self._free_slots[:-n - 1:-1]
+    copies = [[(r.pages[g.index][-1], page, r.length % g.page_size) for page in pages if page is not None] for g, pages in zip(self.paged_groups, fresh)]
+    try:
+      self._copy_on_device(copies, [(r.slot, slot) for slot in slots])
+    except BaseException:
+      for g, pages in zip(self.paged_groups, fresh):
+        g.allocator.free([p for p in pages if p is not None])
+      raise
+    for i, c in enumerate(children):
+      self._requests[c] = self._copy_of(r, self._free_slots.pop(), [pages[i] for pages in fresh])
 
   def reorder(self, parents: Mapping[Hashable, Hashable]) -> None:
     """Every request of ``parents`` goes on from where ``parents[request]`` is, all at once: what a beam search's selection asks for.  The
     parents are requests of the mapping themselves.  A parent's pages and states pass on to one child as they lie; further children get copies
-    as by ``fork``, in the places of the requests that nobody goes on from, whose pages go back.  ``OutOfPages`` changes nothing."""
+    as by ``fork``, in the places of the requests that nobody goes on from, whose pages go back.  ``OutOfPages`` changes nothing; nor does an error of the
+    copies' launches, but that what the requests that nobody goes on from held may have been written over by then."""
     old = {q: self._settled(q) for q in parents}
     if any(p not in old for p in parents.values()):
       raise KeyError("a parent is not among the requests that are reordered")
@@ -476,28 +479,41 @@ class KVCacheManager:
         heir[parent] = child
     dropped = [old[q] for q in parents if q not in heir]
     extra = [(child, parent) for child, parent in parents.items() if heir[parent] != child]
-    for g in self.paged_groups:
+    fresh: List[list] = []      # pages for the copies: free ones, then those that only dropped requests hold
+    reused: List[list] = []
+    wants = [[old[parent].length % g.page_size != 0 for _, parent in extra] for g in self.paged_groups]
+    for g, want in zip(self.paged_groups, wants):
       lost = Counter(p for r in dropped for p in r.pages[g.index] if p)
-      room = g.allocator.num_free + sum(g.allocator.holders(p) == k for p, k in lost.items())
-      # a full page of a dropped request that a copy shares stays held: only pages that no parent holds come back
-      want = sum(1 for _, parent in extra if old[parent].length % g.page_size)
-      if want > room:
-        raise OutOfPages(f"group {g.index}: {want} pages wanted for copies, {room} of {g.num_pages} free")
+      # a full page of a dropped request that a parent holds too stays held: only pages that no parent holds can be had
+      coming = [p for p, k in lost.items() if g.allocator.holders(p) == k]
+      if sum(want) > g.allocator.num_free + len(coming):
+        raise OutOfPages(f"group {g.index}: {sum(want)} pages wanted for copies, {g.allocator.num_free + len(coming)} of {g.num_pages} free")
+      reused.append(coming[:max(0, sum(want) - g.allocator.num_free)])
+    for g, want, again in zip(self.paged_groups, wants, reused):
+      pages = iter(g.allocator.alloc(sum(want) - len(again)) + again)
+      fresh.append([next(pages) if w else None for w in want])
+    copies = [[(old[parent].pages[g.index][-1], page, old[parent].length % g.page_size) for (_, parent), page in zip(extra, pages) if page is not None]
+              for g, pages in zip(self.paged_groups, fresh)]
+    try:
+      self._copy_on_device(copies, [(old[parent].slot, r.slot) for (_, parent), r in zip(extra, dropped)])
+    except BaseException:
+      for g, pages, again in zip(self.paged_groups, fresh, reused):
+        g.allocator.free([p for p in pages if p is not None and p not in again])
+      raise
+    for g, again in zip(self.paged_groups, reused):
+      g.allocator.share(again)      # (for the copies; the dropped requests let go of them now)
     for r in dropped:
       self._give_back(r)
     for parent, child in heir.items():
       self._requests[child] = old[parent]
-    copies: List[List[tuple]] = [[] for _ in self.paged_groups]
-    slots = []
-    for (child, parent), r in zip(extra, dropped):
-      self._requests[child] = self._copy_of(old[parent], r.slot, copies)
-      slots.append((old[parent].slot, r.slot))
-    self._copy_on_device(copies, slots)
+    for i, ((child, parent), r) in enumerate(zip(extra, dropped)):
+      self._requests[child] = self._copy_of(old[parent], r.slot, [pages[i] for pages in fresh])
 
   def keep(self, kept: Mapping[Hashable, Sequence[int]]) -> None:
     """Of the tokens that were appended to each request - the nodes of a drafted tree - those numbered in ``kept`` (rising, from 0) become
     part of it: their keys and values move to the front, one launch a group for all requests, the tokens are committed, and what the others held
-    goes back.  States cannot be kept in part: with groups of states only a beginning of all tokens can stay, which is all of them."""
+    goes back.  States cannot be kept in part: with groups of states only a beginning of all tokens can stay, which is all of them.  An
+    error of the launches commits nothing, but may have moved some of the tokens, which are to be cancelled then."""
     for req_id, nodes in kept.items():
       n = self._requests[req_id].reserved
       if any(not 0 <= a < n for a in nodes) or any(a >= b for a, b in zip(nodes, list(nodes)[1:])):

@@ -209,3 +209,64 @@ def test_more_copies_than_go_in_one_call(monkeypatch):
     seqs[q] = seqs[q] + [10 + q]
   m.reorder({q: 4 + q % 2 for q in range(9)})
   check(m, {q: seqs[4 + q % 2] for q in range(9)})
+
+
+@pytest.mark.parametrize("fails", ["copy_cache_pages", "copy_cache_pages, the second group", "reorder_states"])
+@pytest.mark.parametrize("pages", [40, 10])
+def test_an_error_of_a_launch_leaves_the_requests_as_they_were(pages, fails, monkeypatch):
+  from miniinfer_b200.kernels import ops
+  m = make(window=6, pages=pages, seqs=5, state=True)
+  seqs = {}
+  for q, n in (("a", 5), ("b", 9), ("c", 2)):
+    m.admit(q)
+    seqs[q] = [100 * len(seqs) + i for i in range(n)]
+    write(m, q, seqs[q])
+    m.commit(q, n)
+
+  def everything():
+    return (m.free_pages(), sorted(m._free_slots), [g.block_table_host.copy().tolist() for g in m.paged_groups], [list(g.allocator._held) for g in m.paged_groups],
+            {q: (r.slot, r.length, r.reserved, [list(p) for p in r.pages]) for q, r in m._requests.items()})
+
+  name, plain, left = fails.split(",")[0], getattr(ops, fails.split(",")[0]), [1 if "second" in fails else 0]
+
+  def failing(*args):
+    if not left[0]:
+      raise ops.KernelError("a launch failed")
+    left[0] -= 1
+    plain(*args)
+
+  before = everything()
+  for call in (lambda: m.fork("b", ["d", "e"]), lambda: m.reorder({"a": "b", "b": "b", "c": "a"})):
+    with monkeypatch.context() as patch:
+      patch.setattr(ops, name, failing)
+      left[0] = 1 if "second" in fails else 0
+      with pytest.raises(ops.KernelError):
+        call()
+    assert everything() == before
+    m.check_invariants()
+  for q in "ab":      # what a request goes on from is as it was
+    check(m, {q: seqs[q]})
+  m.reorder({"a": "b", "b": "b", "c": "a"})
+  seqs = {"a": seqs["b"], "b": seqs["b"], "c": seqs["a"]}
+  check(m, seqs)
+  for q in "abc":
+    m.release_request(q)
+  assert m.free_pages() == [g.num_pages for g in m.paged_groups]
+
+
+def test_copies_go_into_the_pages_that_come_back():
+  m = make(pages=4, seqs=3)
+  seqs = {"a": [1, 2, 3, 4, 5], "b": [6, 7], "c": [8]}
+  for q, tokens in seqs.items():
+    m.admit(q)
+    write(m, q, tokens)
+    m.commit(q, len(tokens))
+  assert m.free_pages() == [0]
+  m.reorder({"a": "a", "b": "a", "c": "a"})
+  check(m, {q: seqs["a"] for q in "abc"})
+  assert m.free_pages() == [0]
+  m.release_request("c")
+  m.fork("a", ["d"])
+  check(m, {q: seqs["a"] for q in "abd"})
+  with pytest.raises(OutOfPages):
+    m.append("a", 4)
