@@ -151,7 +151,7 @@ struct Args {
   float2* sums;                  // [R, stretches]: maximum, sum of exp(x - maximum)
   uint64_t* best;                // [R, stretches, n]: keys, 0 where there is none
   double2* norm;                 // [R]: the maximum, cum minus the log of the sum
-  int* arrivals;                 // [requests], zero; left zero
+  int* arrivals;                 // [requests + 1], zero; left zero: blocks of a request that have come, and of all rows
   int R, V, requests, n, stretches, tiles;      // tiles of a stretch
 };
 
@@ -216,6 +216,20 @@ __device__ __forceinline__ void read_tile(float (&v)[ITEMS], const unsigned char
   }
 }
 
+// A block has come, one of all: the last finds all others before it.  (The counter goes back to zero by itself.)
+__device__ __forceinline__ bool last_of_all(const Args& a) {
+  const unsigned others = gridDim.x * a.R - 1;
+  return atomicInc(reinterpret_cast<unsigned*>(&a.arrivals[a.requests]), others) == others;
+}
+// The very last of all blocks leaves the requests' counters at zero, also where a list that does not rise has sent a request fewer blocks than it counts
+// on.  (Up to `step` requests without a loop, whose instructions would have to be fetched: 64 requests 45.2 us, with a loop alone 45.6, without all this 44.7.)
+__device__ __forceinline__ void clear_counters(const Args& a, int first, int step) {
+  if (first < a.requests) a.arrivals[first] = 0;
+  if (a.requests > step)
+#pragma unroll 1
+    for (int q = first + step; q < a.requests; q += step) a.arrivals[q] = 0;
+}
+
 // Puts a request's pieces together; by the whole block.  `stages`: NEAR candidates' keys and images.  `shared`: room for `room` candidates' images, keys
 // and rows.  A candidate's order: the score's image, then the lower row, then the row's key.
 constexpr int NEAR = 4096;
@@ -229,6 +243,7 @@ __device__ __noinline__ void finish(const Args& a, int request, int r0, int r1, 
   auto sums_of = [&](int r) { return r < r1 && lane < a.stretches ? __ldcg(&a.sums[(size_t)r * a.stretches + lane]) : make_float2(-INFINITY, 0.f); };
   float2 near = sums_of(r0 + warp);
   float cum = r0 + warp < r1 ? a.cum[r0 + warp] : 0.f;
+  const bool last = threadIdx.x == 0 && last_of_all(a);      // (on its way beside the loads)
 #pragma unroll 4
   for (int i = threadIdx.x; i < min(total, NEAR); i += THREADS) near_key[i] = __ldcg(place_of(i));
 #pragma unroll 1
@@ -251,7 +266,7 @@ __device__ __noinline__ void finish(const Args& a, int request, int r0, int r1, 
     if (lane == 0) a.norm[r] = make_double2((double)m, (double)cum - log(s));
   }
   if (threadIdx.x == 0) *count = 0;
-  __syncthreads();
+  if (__syncthreads_or(last)) clear_counters(a, threadIdx.x, THREADS);
   auto row_of = [&](int i) { return r0 + i % pieces / a.stretches; };
   auto score_image = [&](int i, uint64_t key) {      // 0: no candidate
     if (key == 0) return (uint64_t)0;
@@ -558,7 +573,17 @@ beam_select_kernel(Args a) {
     }
   }
   __syncthreads();
-  if (!s_last) return;
+  if (!s_last) {
+    if (warp == 0) {
+      bool last = false;
+      if (lane == 0) {
+        __threadfence();
+        last = last_of_all(a);
+      }
+      if (__shfl_sync(FULL, last, 0)) clear_counters(a, lane, 32);
+    }
+    return;
+  }
   __threadfence();
   finish(a, s_request, s_rows[0], s_rows[1], of_warp, stages, reinterpret_cast<unsigned char*>(pool), ROOM * 8 / 20, lists, &s_nth, &s_count);
 }
@@ -595,7 +620,7 @@ MI_API long long mi_beam_select_words(int R, int V, int n) {
   return (long long)R * ((V + per - 1) / per) * (n + 1) + 2ll * R + 1;
 }
 
-// scratch: mi_beam_select_words words, 8-byte aligned; arrivals: one zero word a request, left zero.
+// scratch: mi_beam_select_words words, 8-byte aligned; arrivals: one zero word a request and one more, left zero.
 MI_API int mi_beam_select(int* tokens, int* parents, float* scores, const void* logits, int dtype, const float* cum, const int* start, void* scratch,
                           int* arrivals, int R, int V, int requests, int n, cudaStream_t stream) {
   MI_REQUIRE(R >= 0 && V > 0 && requests >= 0 && n >= 1 && n <= MAX_BEST, "beam_select: bad sizes R=%d V=%d requests=%d n=%d (n is at most %d)", R, V, requests, n, MAX_BEST);

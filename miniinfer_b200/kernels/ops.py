@@ -1390,10 +1390,10 @@ def beam_select(tokens: torch.Tensor, parents: torch.Tensor, scores: torch.Tenso
   words = int(_entry("mi_beam_select_words", "iii", "l")(R, V, n))
   if workspace is not None:
     scratch = workspace.buffer("beam_scratch", (words,), torch.int64)
-    arrivals = workspace.zeros("beam_arrivals", requests, torch.int32)
+    arrivals = workspace.zeros("beam_arrivals", requests + 1, torch.int32)
   else:
     scratch = torch.empty(words, dtype=torch.int64, device=logits.device)
-    arrivals = torch.zeros(requests, dtype=torch.int32, device=logits.device)
+    arrivals = torch.zeros(requests + 1, dtype=torch.int32, device=logits.device)
   _check(common_lib(), _entry("mi_beam_select", "ppppipppp" + "iiiip")(
     at(tokens, torch.int32), at(parents, torch.int32), at(scores, torch.float32), at(logits, logits.dtype), dt, at(cum, torch.float32),
     at(row_start, torch.int32), at(scratch, torch.int64), at(arrivals, torch.int32), R, V, requests, n, _current_stream(device)))

@@ -194,3 +194,19 @@ def test_many_rows_whose_best_come_early_or_late(n, V):
   cum = cum + torch.arange(len(logits), device=DEV) * 10      # (so that rows do not tie)
   for start in (list(range(len(logits) + 1)), [0, 12, 24, 36, len(logits)]):
     check(select(logits, cum, start, n), logits, cum, start, n)
+
+
+def test_a_list_that_does_not_rise_harms_no_later_call():
+  """What such a call answers is open; the counters of the workspace that it shares with later ones are left as every call finds them."""
+  from miniinfer_b200.engine.context import Workspace
+  if DEV == "cpu":
+    pytest.skip("counters")
+  g = torch.Generator().manual_seed(3)
+  logits, cum = torch.randn((8, 40000), generator=g).to(DEV), torch.zeros(8, device=DEV)
+  for bad in ([0, 5, 2, 8], [4, 0, 8], [0, 3, 1, 6, 8], [8, 6, 4, 2, 0]):
+    ws = Workspace(DEV)
+    select(logits, cum, [0, 2, 4, 6, 8], 5, ws)
+    select(logits, cum, bad, 5, ws)
+    assert not ws._bufs[("beam_arrivals", torch.int32)].any()
+    for start in ([0, 4, 8], [0, 2, 3, 8], [0, 2, 4, 6, 8]):
+      check(select(logits, cum, start, 5, ws), logits, cum, start, 5)
