@@ -75,6 +75,17 @@ __device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, volati
   *abort = 1;
   atomicExch(status, 2);
 }
+// The wait at a role's end: what it has started itself, copies or products, is over before the block is.  It does not ask for `abort`, but has a limit too.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  for (int i = 0; i < WAIT_LIMIT; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+    if (done) return;
+  }
+}
 __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -379,6 +390,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* spoiled = abort + 1;      // [2]: the last piece, by parity, in which a value was not finite
   volatile int* last_to_come = spoiled + 2;
+  uint64_t* drained = bars + 43;        // the last products are done
   Piece* pieces = reinterpret_cast<Piece*>(bars + 44);
   float2* of_set = reinterpret_cast<float2*>(bars + BARS);      // [2][BM]: a row's maximum and sum in each stream of keys, at a piece's end
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -386,6 +398,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     mbar_init(o_free, SOFTMAX_WARPS);
+    mbar_init(drained, 1);
     for (int u = 0; u < k.ring; ++u) {
       mbar_init(&u_full[u], 1);
       mbar_init(&u_empty[u], 1);
@@ -465,6 +478,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
     const int rows = k.tokens * a.G;
     int4 joined = make_int4(0, 0, 0, 0);      // for the kernel that joins pieces
     int slot = 0, turn = 1, it = 0;      // the ring's next unit; the parity that its barrier of free units is waited with
+    int units = 0;                       // asked for so far
     auto stopped = [&]() { return __shfl_sync(0xffffffffu, *abort, 0) != 0; };      // the same answer for all lanes, which go on together
     for (;; ++it) {
       Piece p;
@@ -494,13 +508,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       auto load = [&](int j, int page_id, int which) {
         const int s = slot;
         mbar_wait(&u_empty[s], (uint32_t)turn, abort, k.status);
+        if (stopped()) return;      // (all lanes or none: a unit whose boxes are not all on their way would never be full)
         if (++slot == k.ring) {
           slot = 0;
           turn ^= 1;
         }
+        ++units;
         if (lane == 0) mbar_expect_tx(&u_full[s], (uint32_t)unit_bytes);
         __syncwarp();
-        if (lane < loads && !*abort) {
+        if (lane < loads) {
           const int key = p.key + j * BN + row;
           const int y = ((page_id * 2 + which) * a.nkv + p.head) * a.page_size + key % a.page_size;      // (fits: the launcher asks for it)
           tma_load(ring_s + s * unit_bytes + column * COL_BYTES + row * 128, &kv_map, column * BOX, y, &u_full[s]);
@@ -520,6 +536,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       }
     }
     if (lane == 0) k.joins[me] = joined;
+    // no copy is on its way into this block's memory when the block ends, also where a wait has run out
+    for (int u = max(units - k.ring, 0); u < units; ++u) mbar_drain(&u_full[u % k.ring], (uint32_t)(u / k.ring & 1));
+    if (it > 0) mbar_drain(q_full, (uint32_t)(it - 1) & 1);
   } else if (warp == MMA_WARP) {
     {      // the whole warp goes through the waits together, one elected thread issues: descriptors then stay in uniform registers
       auto stopped = [&]() { return __shfl_sync(0xffffffffu, *abort, 0) != 0; };
@@ -636,6 +655,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         }
         if constexpr (QT == 2) done[0] += n;
       }
+      commit(drained);      // nor does a product read it, or write tensor memory that goes back
+      mbar_drain(drained, 0);
     }
   } else if (warp < SOFTMAX_WARPS) {
     // Warp w: set w / 4, tensor-memory lanes 32 (w % 4) .. + 31, a thread a row.
