@@ -36,6 +36,7 @@ constexpr int BM = 128, BOX = 64, BUFFERS = 2;
 constexpr int TMEM_COLS = 512, S_COL = 256;
 constexpr int MAX_UNITS = 12;                 // boxes of the ring: a tile's keys or its values each
 constexpr int WAIT_LIMIT = 1 << 22;
+constexpr int STATUS_LATE = 64, STATUS_PLACE = 128;      // bits of the status word: a bounded wait ran out; shared memory is not laid out as the kernel needs it
 constexpr int SMEM_BYTES = 227 << 10;
 constexpr int BARS = 80;                      // 8-byte words behind queries and ring: barriers, pieces
 
@@ -73,7 +74,7 @@ __device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, volati
     if ((i & 63) == 63 && *abort) return;
   }
   *abort = 1;
-  atomicExch(status, 2);
+  atomicOr(status, STATUS_LATE);
 }
 // The wait at a role's end: what it has started itself, copies or products, is over before the block is.  It does not ask for `abort`, but has a limit too.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
@@ -374,7 +375,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
   if (smem_u32(smem) & 1023u) {
     mi::grid_dependency_sync();
     if (threadIdx.x == 0) {
-      atomicExch(k.status, 4);
+      atomicOr(k.status, STATUS_PLACE);
       k.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
     return;
@@ -960,8 +961,8 @@ MI_API long long mi_attention_tree_tc_floats(int nh, int nkv, int hd, int page_s
 }
 
 // bfloat16.  scratch: mi_attention_tree_tc_floats floats, 16-byte aligned; counters: a zero word for each item, key/value head and set of
-// 128 / G tokens of max_q, left zero; status: one word, set to 2 if a bounded wait ran out, to 4 if shared memory is
-// not laid out as the kernel needs it.  Answers 2 for sizes or addresses that it does not take.
+// 128 / G tokens of max_q, left zero; status: one word, which gets STATUS_LATE or
+// STATUS_PLACE.  Answers 2 for sizes or addresses that it does not take.
 MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, const int* block_table, int bt_stride, const int* q_start, const int* q_len,
                                 const int* ctx_len, const int* seq_slot, const int* mask, int words, const int* positions, const float* sink, float* scratch,
                                 int* counters, int* status, int items, int T, int width, int nh, int nkv, int hd, int pages, int page_size, int window, int max_q, float scale,

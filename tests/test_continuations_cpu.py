@@ -69,3 +69,26 @@ def test_tree_attention_refuses():
       call(None, change)
   with pytest.raises(KernelError):
     call(dict(window=4), dict(positions=None))
+
+
+@pytest.mark.parametrize("code,name", [(64, "attention over trees"), (128, "its place in shared memory")])
+def test_a_wait_that_ran_out_over_a_tree_is_told_from_those_of_other_kernels(code, name):
+  """A bit of its own for each: 2 is the prefill attention's, 4 the tcgen05 matrix product's."""
+  import os
+  import re
+  from types import SimpleNamespace
+
+  from miniinfer_b200.engine.context import Workspace
+  from miniinfer_b200.engine.runner import ModelRunner
+  from miniinfer_b200.kernels import build
+  source = open(os.path.join(build.CSRC, "attention_tree_tc.cu"), encoding="utf-8").read()
+  bits = dict(re.findall(r"(STATUS_\w+) = (\d+)", source))
+  assert str(code) in bits.values()
+  assert set(re.findall(r"atomic(?:Exch|Or)\(\w*\.?status, (\w+)\)", source)) == set(bits)      # the kernel sets these and no others
+  ws = Workspace(torch.device("cpu"))
+  word = ws.zeros("attention_tree_status", 1, torch.int32)
+  runner = SimpleNamespace(ws=ws, _graphs={}, _step_graphs={})
+  ModelRunner.check_status(runner)
+  word[0] = code
+  with pytest.raises(KernelError, match=f"status bits {code}:.* {code} {name}"):
+    ModelRunner.check_status(runner)
