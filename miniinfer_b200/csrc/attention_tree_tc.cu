@@ -361,6 +361,22 @@ __device__ __forceinline__ void join_row(const Tc& k, int first, const int4& u, 
                                                           pack_bf16(acc[f + 1][0] * inv, acc[f + 1][1] * inv), pack_bf16(acc[f + 1][2] * inv, acc[f + 1][3] * inv));
 }
 
+// A wait has run out here, or in a call before that shared the counters, which are then not what they should be: all rows become NaN, and
+// so do the sums that this block owes to those who join them.
+template <int QT>
+__device__ __forceinline__ void give_up(const Tc& k) {
+  const Args& a = k.a;
+#pragma unroll 1
+  for (int b = 0; b < a.items; ++b) {
+    const Item it = item_of(a, b);
+    __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)it.row0 * a.nh * a.hd;
+#pragma unroll 1
+    for (size_t i = threadIdx.x; i < (size_t)it.n * a.nh * a.hd; i += blockDim.x) rows[i] = __float2bfloat16(NAN);
+  }
+#pragma unroll 1
+  for (int i = threadIdx.x; i < 2 * QT * BM; i += blockDim.x) reinterpret_cast<float2*>(a.part_ml)[(size_t)2 * blockIdx.x * QT * BM + i] = make_float2(NAN, NAN);
+}
+
 constexpr int threads_of(int sets) { return 32 * (4 * sets + 2); }
 
 template <int QT, int SETS, int BN, int STEPS>
@@ -378,6 +394,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       atomicOr(k.status, STATUS_PLACE);
       k.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
+    give_up<QT>(k);
     return;
   }
   const int q_bytes = k.boxes * Q_COL_BYTES, unit_bytes = k.boxes * COL_BYTES;      // of a set of rows; of a tile's keys or values
@@ -428,6 +445,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
   auto value_unit = [](int j, int n) { return KEYS ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; };
 
   if (warp == PRODUCER_WARP) {
+    const int late = lane == 0 ? *reinterpret_cast<volatile int*>(k.status) : 0;      // (on its way beside the items' sizes)
     // where this block's stretch of the line begins
     int overhead = 0;
     auto places_of = [&](const Item& it) {
@@ -481,10 +499,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
     int slot = 0, turn = 1, it = 0;      // the ring's next unit; the parity that its barrier of free units is waited with
     int units = 0;                       // asked for so far
     auto stopped = [&]() { return __shfl_sync(0xffffffffu, *abort, 0) != 0; };      // the same answer for all lanes, which go on together
+    const bool lost = __shfl_sync(0xffffffffu, late, 0) != 0;
     for (;; ++it) {
       Piece p;
-      const bool more_pieces = walk.next(p);
+      const bool more_pieces = !lost && walk.next(p);
       if (!more_pieces) p.n = 0;
+      if (lost) *abort = 1;
       const int* bt = p.it.bt;
       const int row = lane / k.boxes * k.box_rows, column = lane % k.boxes;
       auto page_at = [&](int j) {
@@ -493,7 +513,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       };
       int page = page_at(0), behind = 0;
       mbar_wait(q_empty, (it & 1) ^ 1, abort, k.status);
-      if (stopped()) break;
+      if (stopped() && !lost) break;
       if (lane == 0) {
         pieces[it % PIECES] = p;
         mbar_arrive(&piece_full[it % PIECES]);
@@ -884,6 +904,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
   // every tensor-memory access is done, then the columns go back
   tc_fence_before();
   __syncthreads();
+  if (*abort) give_up<QT>(k);
   if (warp == MMA_WARP) {
     __syncwarp();
     tc_fence_after();

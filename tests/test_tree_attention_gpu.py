@@ -212,3 +212,29 @@ def test_pages_beyond_32_bits_of_a_cache(dtype):
   got = torch.empty_like(want)
   ops.tree_attention(got, qkv, large, table + (pages - kv.shape[0]), batch, 16, 8, 128, 128 ** -0.5)
   assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("case", [3, 4, 6])
+def test_a_workspace_in_which_a_wait_has_run_out_gives_no_numbers(case):
+  """Its counters may be off then: rows become NaN instead of sums of some of their pieces, rows of no item stay, and the status says it again."""
+  from miniinfer_b200.engine.context import Workspace
+  from miniinfer_b200.kernels import ops
+  if DEV == "cpu":
+    pytest.skip("a status word")
+  ws = Workspace(DEV)
+  out, args = run(case, torch.bfloat16, scratch=ws, gap=2)
+  want = out.clone()
+  batch = args[3]
+  mine = torch.zeros(out.shape[0], dtype=torch.bool)
+  for s, n in zip(batch.q_start.tolist(), batch.q_len.tolist()):
+    mine[s:s + n] = True
+  assert torch.isfinite(want[mine.to(DEV)]).all() and ops.device_status(ws) == 0
+  word = ws.zeros("attention_tree_status", 1, torch.int32)
+  word[0] = 64      # as a call leaves it whose wait has run out
+  out.fill_(777.0)
+  ops.tree_attention(out, *args)
+  assert torch.isnan(out[mine.to(DEV)]).all() and (out[~mine.to(DEV)] == 777.0).all()
+  assert ops.device_status(ws) == 64
+  word[0] = 0
+  ops.tree_attention(out, *args)
+  assert torch.equal(out, want)
