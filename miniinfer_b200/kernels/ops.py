@@ -1652,7 +1652,9 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
   on top of the context's length: one of the places that the item's new tokens have).  ``sink`` and ``softcap`` as in ``attention``.  A row that sees nothing becomes zero; rows of no item stay as they were.
 
   Of ``batch`` it reads ``q_start, q_len, ctx_len, seq_slot`` and ``tree_mask`` (int32; ``positions`` too with a window), ``num_items``,
-  ``max_q_len`` - no item has more new tokens -, ``max_ctx_len`` and ``scratch``."""
+  ``max_q_len`` - no item has more new tokens -, ``max_ctx_len`` and ``scratch``: a ``Workspace``, which one call uses at a time.  Without it a
+  bfloat16 call waits for the device, to see that no bounded wait has run out, and cannot be captured; with it ``device_status`` tells, and from
+  then on the workspace gives NaN."""
   T, mask = qkv.shape[0], batch.tree_mask
   if num_kv_heads < 1 or num_heads % num_kv_heads or not 0 < head_dim <= MAX_HEAD_DIM:
     raise KernelError(f"tree_attention: {num_heads} heads over {num_kv_heads} of {head_dim}")
@@ -1694,6 +1696,8 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
       scratch = ws.buffer("attention_tree_partials", (n,), torch.float32)
       counters, status = ws.zeros("attention_tree_counters", units, torch.int32), ws.zeros("attention_tree_status", 1, torch.int32)
     else:
+      if torch.cuda.is_current_stream_capturing():
+        raise KernelError("tree_attention: a call without a workspace waits for the device and cannot be captured")
       scratch = torch.empty(n, dtype=torch.float32, device=qkv.device)
       counters, status = torch.zeros(units, dtype=torch.int32, device=qkv.device), torch.zeros(1, dtype=torch.int32, device=qkv.device)
     code = _entry("mi_attention_tree_tc", "ppppi" + "ppppp" + "ipppppi" + "iiiiiiiiiffp")(

@@ -238,3 +238,16 @@ def test_a_workspace_in_which_a_wait_has_run_out_gives_no_numbers(case):
   word[0] = 0
   ops.tree_attention(out, *args)
   assert torch.equal(out, want)
+
+
+def test_a_call_without_a_workspace_is_not_captured():
+  from miniinfer_b200.kernels import ops
+  if DEV == "cpu":
+    pytest.skip("graphs")
+  want, args = run(3, torch.bfloat16)
+  out = torch.zeros_like(want)
+  with pytest.raises(ops.KernelError, match="captured"):
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+      ops.tree_attention(out, *args)
+  ops.tree_attention(out, *args)
+  assert torch.equal(out, want)
