@@ -936,6 +936,8 @@ EncodeFn encoder() {
   return fn;
 }
 
+constexpr int NOT_TAKEN = 2, JOINED = 3;      // answers beside 0 and 1: another kernel's sizes; two launches, the second of which joins the pieces
+
 template <int QT, int SETS, int BN, int STEPS>
 int launch(Tc& k, const CUtensorMap& q_map, const CUtensorMap& kv_map, int blocks, cudaStream_t stream) {
   static bool ready[64] = {};
@@ -963,7 +965,7 @@ int launch(Tc& k, const CUtensorMap& q_map, const CUtensorMap& kv_map, int block
   if (mi::launch(join, dim3(blocks, QT, columns), dim3(32 * JOIN_WARPS), 0, stream, k) != cudaSuccess)
     return mi_fail("attention_tree_tc: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   MI_LAUNCH_OK("attention_tree_tc");
-  return 0;
+  return JOINED;
 }
 
 // (8 rows in 20 pieces a unit, 164 KB: 16.6 us on the device either way, and 5 us less to launch; 96 rows in 4 pieces, 256 KB: 31 against 24 us)
@@ -983,7 +985,7 @@ MI_API long long mi_attention_tree_tc_floats(int nh, int nkv, int hd, int page_s
 
 // bfloat16.  scratch: mi_attention_tree_tc_floats floats, 16-byte aligned; counters: a zero word for each item, key/value head and set of
 // 128 / G tokens of max_q, left zero; status: one word, which gets STATUS_LATE or
-// STATUS_PLACE.  Answers 2 for sizes or addresses that it does not take.
+// STATUS_PLACE.  Answers NOT_TAKEN for sizes or addresses that it does not take, JOINED if it has launched two kernels instead of one.
 MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, const int* block_table, int bt_stride, const int* q_start, const int* q_len,
                                 const int* ctx_len, const int* seq_slot, const int* mask, int words, const int* positions, const float* sink, float* scratch,
                                 int* counters, int* status, int items, int T, int width, int nh, int nkv, int hd, int pages, int page_size, int window, int max_q, float scale,
@@ -992,7 +994,7 @@ MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, cons
   if (mi_attention_tree_tc_floats(nh, nkv, hd, page_size, max_q) == 0 || width % 8 != 0 || !(scale > 0.f) || T == 0 ||
       ((uintptr_t)out | (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)scratch) % 16 != 0 || (long long)pages * 2 * nkv * page_size > 0x7fffffffll ||
       ((long long)bt_stride * page_size / 64 + 2 + OVERHEAD) * items * nkv * (max_q / (BM / (nh / nkv)) + 1) > 0x7fffffffll)      // the last: the line of tiles
-    return 2;
+    return NOT_TAKEN;
   if (items == 0) return 0;
   const EncodeFn encode = encoder();
   if (!encode) return mi_fail("attention_tree_tc: the driver does not offer cuTensorMapEncodeTiled");

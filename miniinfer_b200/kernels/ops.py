@@ -1703,7 +1703,7 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
     code = _entry("mi_attention_tree_tc", "ppppi" + "ppppp" + "ipppppi" + "iiiiiiiiiffp")(
       *head, *where, scratch.data_ptr(), counters.data_ptr(), status.data_ptr(), *sizes, stream)
     if code != TREE_NOT_TAKEN:
-      _check(common_lib(), code)      # (one more where a kernel of its own joins the pieces)
+      _check(common_lib(), 0 if code == TREE_JOINED else code, kernels=1 + int(code == TREE_JOINED))
       if ws is None and int(status[0]) != 0:
         raise KernelError("tree_attention: a bounded wait on a barrier ran out")
       return
@@ -1722,6 +1722,7 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
 
 
 TREE_NOT_TAKEN = 2      # what mi_attention_tree_tc answers for sizes or addresses that it leaves to mi_attention_tree
+TREE_JOINED = 3         # and where a kernel of its own has joined the pieces
 _tree_floats: Dict[tuple, int] = {}
 
 

@@ -251,3 +251,15 @@ def test_a_call_without_a_workspace_is_not_captured():
       ops.tree_attention(out, *args)
   ops.tree_attention(out, *args)
   assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("case,dtype,kernels", [(3, torch.bfloat16, 1), (5, torch.bfloat16, 2), (10, torch.bfloat16, 2), (3, torch.float32, 2), (0, torch.float32, 1)])
+def test_the_launches_of_a_call_are_counted(case, dtype, kernels):
+  """One kernel, or two where another one joins the pieces: in bfloat16 where a unit's rows are many, in float32 wherever there are pieces."""
+  from miniinfer_b200.kernels import ops
+  if DEV == "cpu":
+    pytest.skip("launches")
+  out, args = run(case, dtype)
+  before = ops.launch_count()
+  ops.tree_attention(out, *args)
+  assert ops.launch_count() - before == kernels
