@@ -881,7 +881,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
-      if (QT == 1 && !whole && k.counters) {      // few rows: the unit's last piece to come joins them all, a launch less
+      if (KEYS && !whole && k.counters) {      // few rows: the unit's last piece to come joins them all, a launch less
         __threadfence();
         sync_softmax();
         if (threadIdx.x == 0) {
@@ -968,7 +968,11 @@ int launch(Tc& k, const CUtensorMap& q_map, const CUtensorMap& kv_map, int block
   return JOINED;
 }
 
-// (8 rows in 20 pieces a unit, 164 KB: 16.6 us on the device either way, and 5 us less to launch; 96 rows in 4 pieces, 256 KB: 31 against 24 us)
+// A unit's last block to come joins its pieces where that is a moment's work for one block: 32 rows, of heads that leave it both sets of softmax
+// warps, and so many bytes.  On the device, inside and by a kernel of its own (which takes a launch, 5 us of the host's time, more): 8 requests, groups of 4,
+// 4 pieces of 16, 32, 48, 96 rows of 128 columns 23.9, 23.7, 25.9, 29.2 and 23.9, 24.0, 24.6, 25.5 us; one request, groups of 2, 20 pieces of 8, 16, 32, 64
+// rows (80 KB to 640) 16.2, 16.6, 17.5, 23.9 and 16.4 to 16.7, of 64 columns 12.7, 13.0, 13.5, 16.9 and 15.0 to 15.4, of 256 columns 43 and 24.7.
+constexpr int JOIN_INSIDE_ROWS = 32;
 constexpr long long JOIN_INSIDE_BYTES = 192 << 10;
 
 // Sets of 128 rows that a block takes at a time: two once the largest item has more rows than one holds, as far as tensor memory goes.
@@ -1013,7 +1017,7 @@ MI_API int mi_attention_tree_tc(void* out, const void* qkv, const void* kv, cons
   const int blocks = mi::sm_count();
   // Pieces are joined by the unit's last block to come, a launch less, where that is little for one block to do; else by a kernel of their own.
   const long long units = (long long)items * nkv * k.max_parts, rows = (long long)max_q * G, pieces = blocks / units + 2;
-  k.counters = qt == 1 && rows <= BM && pieces * rows * hd * 4 <= JOIN_INSIDE_BYTES ? counters : nullptr;
+  k.counters = hd <= 128 && rows <= JOIN_INSIDE_ROWS && pieces * rows * hd * 4 <= JOIN_INSIDE_BYTES ? counters : nullptr;
   k.joins = (int4*)scratch;
   float* part_o = scratch + 4ll * blocks;
   float* part_ml = part_o + 2ll * blocks * qt * BM * k.n_out;
