@@ -106,3 +106,11 @@ def test_a_window_that_leaves_some_rows_a_key_or_two_of_the_first_tile(past, n, 
 @pytest.mark.parametrize("hd", [64, 256])
 def test_in_32_bits(hd, n, kind):
   check([700, 1300], (2, 4), hd, n, kind, torch.float32)
+
+
+@pytest.mark.parametrize("kind", ["planted", "rising"])
+@pytest.mark.parametrize("n", [1, 3, 8])
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+def test_few_rows_whose_pieces_the_last_block_joins(hd, n, kind):
+  """Up to 32 rows of heads up to 128, beside heads of 256, whose pieces another kernel joins."""
+  check(SPLIT[:2], (8, 4), hd, n, kind, torch.bfloat16)
