@@ -8,12 +8,15 @@
 // tile's keys are dealt out to several warps a row group, each with an online softmax of its own, put together at the end of the piece.  Pieces give
 // a small step enough blocks; more than one of them leave sums that tree_merge_kernel puts together.
 //
+// How many pieces there are follows from the step's items, longest context and the SMs, how many warps share a row from the largest item: unlike
+// attention_f32.cu, whose segments are fixed, the last bits of a row may differ with what else is in the batch, within the bound that the tests derive.
+//
 // A key that a row does not see has the weight -1, which the weighted values leave out: a zero would make a NaN of an infinity there.
 //
 // What bounds it: shared memory, whose 16 bytes of a key or value serve four rows - 16 FMAs a lane to five wavefronts and more, where the FMAs take four
 // cycles -, and with few rows the fetching of tiles, of which a block has one on its way.  Measured in float32: 3 trees of 13 over about 1000 keys, 16 heads on
 // 8, 22 us (the bytes 2.2); 8 single tokens over 4000 keys 82 us, 49 % of the bytes' rate (135 with all of a row's keys in one warp); 8 trees of 8 over 2000
-// keys 81 us, the FMAs 15.
+// keys 81 us, the FMAs 15.  In bf16, with pages of 24 that the tensor-core kernel leaves to this one, 8 trees of 32 over up to 4096 keys, 32 heads on 8, 441 us.
 #include "attention_tree.cuh"
 
 namespace {

@@ -19,9 +19,10 @@
 // Weights are relative to a maximum that may lag behind the row's by 2^8, so that a row of sums is rescaled a few times and not in every tile; they are
 // rounded to bf16, as the tensor cores take them, and the sum that divides the row is that of the rounded ones.
 //
-// Measured, heads of 128: 32 trees of 64 over up to 8192 keys, 32 heads on 8 (625 MB, 105 GFLOP) 180 us, 3.5 TB/s and 0.58 PFLOP/s; 8 trees of 32 over up to
-// 4096 keys (62 MB) 24 us; one tree of 8 over 2047 keys, 16 heads on 8 (8.5 MB) 16.5 us.  The first is bound by the chain from scores over exponentials to
-// weights: two sets of rows leave the tensor cores 35 % busy, without the softmax the products and copies alone took 130 us.  The others are bound by what a
+// Measured, heads of 128: 32 trees of 64 over up to 8192 keys, 32 heads on 8 (625 MB, 105 GFLOP) 180 us in short bursts, 200 to 215 one call after the other (the power cap): 3.5 and 2.9 to 3.1 TB/s; 8 trees of 32 over up to
+// 4096 keys (62 MB) 24 to 26 us, with a cap of 30 37.5, with pages of 16 30.5, heads of 64 and 256 21.8 and 40.3; one tree of 8 over 2047 keys, 16 heads on 8 (8.5 MB) 16.5 us.  The first is
+// bound by the chain from scores over exponentials to weights (with a cap, two more operations of the exponentials' unit a score, 404 us): two sets of rows leave the tensor cores 35 % busy,
+// without the softmax the products and copies alone took 130 us.  The others are bound by what a
 // piece costs whatever its length is - its description, its queries, the first tile's latency, its sums - about 4000 cycles, and 10000 once a block.
 #include <cuda.h>
 #include <string.h>
@@ -181,7 +182,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // The line of work: item after item, in an item head after head, in a head part after part (QT * tokens tokens each).  A unit takes its
 // tiles and `overhead` more in front of them: what queries, the first copies and the results cost, as long as a block has several tiles.
-constexpr int OVERHEAD = 4, OVERHEAD_FROM = 4;      // from that many tiles a block on (32 trees over up to 8192 keys: 208 us; without it 237)
+// From that many tiles a block on.  24 sizes - 4 to 64 requests, trees of 8 to 64, contexts of 512 to 8192, heads of 64 to 256 - without it 2 to 16 % slower in 20, equal
+// in 4; with it from none on 11 % slower at 1 to 3 tiles a block in two, 5 % faster in one.
+constexpr int OVERHEAD = 4, OVERHEAD_FROM = 4;
 struct Line {
   int t_begin, tiles, parts;     // of an item: first tile that some row sees, tiles, parts
 };

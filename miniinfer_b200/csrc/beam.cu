@@ -16,12 +16,14 @@
 // by counting.  Should many more come (equal values, a tile of which a warp has only poor ones or none), the n-th best of the 256 threads'
 // bests is found exactly: at most n times a thread's 16 values are not below that.
 //
-// Float32 holds a value and a piece's sum; normalisers and scores are made in 64 bits, so that candidates of different beams, which may lie
-// closer than a float32 of their size tells apart, are put in the right order.  The score that is handed out is rounded once.
+// Float32 holds a value and a row's sum of exponentials, made by the hardware's exponential: a normaliser errs by up to 3.5e-6 (derived beside the tests).
+// From there on - its logarithm, the scores and their order - all is in 64 bits, and the score that is handed out is rounded once.  So a row's own candidates
+// are always in their order, and those of different beams wherever their scores are further apart than two normalisers may err.
 //
-// Measured: 64 requests, 263 rows of 151936 float32 (160 MB) 45 us, 3.6 TB/s (49 us with a barrier in each tile): the walk itself takes 23 us, the memory's
-// full rate, but 5 us pass before the first tile is ranked and 14 in the last ranking and joining, chains of short steps with nothing on its way.  4 rows of one request 13.4 us for 2.4 MB: that
-// chain and little else.
+// Measured: 64 requests, 263 rows of 151936 float32 (160 MB) 45 us, 3.5 TB/s (49 us with a barrier in each tile): the walk itself takes 23 us, the memory's
+// full rate, but 5 us pass before the first tile is ranked and 14 in the last ranking and joining, chains of short steps with nothing on its way.  4 rows of one request 13.2 to 13.7 us for
+// 2.4 MB: that chain and little else.  In bf16 41 and 13.8 us, bound by the instructions a value takes.  Rows whose bytes are not a multiple of 16 are read value by
+// value, with nothing on its way ahead: 263 rows of 151935 62 us in float32, 119 in bf16.
 #include "attention_scores.cuh"
 #include "common.cuh"
 
@@ -31,7 +33,9 @@ constexpr int THREADS = 256, WARPS = THREADS / 32, ITEMS = 16, TILE = THREADS * 
 constexpr int STAGES = 4;                     // tiles in shared memory: three on their way, one that was just read
 constexpr int MAX_BEST = 128;
 constexpr int ROOM = MAX_BEST * (ITEMS + 1) + 384;      // candidates: the n best so far and a tile's on top; what is over lets a few tiles come before they are thinned out
-constexpr int BLOCKS_WANTED = 1;              // (263 rows of 151936: 48 us; 2, which are one and a half rounds of blocks: 63)
+// (263 rows of 151936: 48 us; 2, which are one and a half rounds of blocks: 63.  As many stretches as two blocks an SM in one round allow: 1 to 7 rows 15 to 56 us instead of 12 to
+// 22, for more pieces take longer to join than the walk gains; 8 and 24 to 48 rows up to 18 % slower or as now, 16 and 64 rows 16.7 and 20.8 instead of 18.9 and 27.0)
+constexpr int BLOCKS_WANTED = 1;
 constexpr int MANY = 256;                     // candidates of a tile that are ranked without a second thought
 constexpr unsigned FULL = 0xffffffffu;
 

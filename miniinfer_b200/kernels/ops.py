@@ -1373,8 +1373,9 @@ def beam_select(tokens: torch.Tensor, parents: torch.Tensor, scores: torch.Tenso
 
   A score that is minus infinity or no number is no candidate: a forbidden token, a beam with ``cum`` minus infinity, a row that holds
   a NaN or plus infinity.  Places that are left get token -1, parent -1 and score minus infinity; so do requests without rows.  n is at
-  most ``BEAM_MAX_BEST``.  Sums and scores are made in 64 bits.  ``workspace`` (a ``Workspace``) lends the scratch; without it scratch is
-  allocated."""
+  most ``BEAM_MAX_BEST``.  A row's sum of exponentials is held in float32, its logarithm and the scores in 64 bits: candidates of different beams
+  are in the order of their scores where these differ by more than two normalisers may err (3.5e-6 each).  ``workspace`` (a ``Workspace``, which
+  one call uses at a time) lends the scratch; without it scratch is allocated."""
   if logits.dim() != 2 or tokens.dim() != 2 or row_start.dim() != 1 or row_start.shape[0] != tokens.shape[0] + 1:
     raise KernelError("beam_select: logits must be [rows, vocabulary], the results [requests, n], row_start [requests + 1]")
   (R, V), (requests, n) = logits.shape, tokens.shape
@@ -1650,6 +1651,7 @@ def tree_attention(out: torch.Tensor, qkv: torch.Tensor, kv_layer: torch.Tensor,
   lie behind the context in the item's pages, in the order of the rows, whatever their positions are.  ``window``: a token at position p
   sees keys of positions above ``p - window`` only; a context key's position is its place, a new token's is ``batch.positions`` (its depth
   on top of the context's length: one of the places that the item's new tokens have).  ``sink`` and ``softcap`` as in ``attention``.  A row that sees nothing becomes zero; rows of no item stay as they were.
+  The last bits of a row may differ with what else is in the batch, which decides how its keys are cut into pieces; the same call gives the same bits.
 
   Of ``batch`` it reads ``q_start, q_len, ctx_len, seq_slot`` and ``tree_mask`` (int32; ``positions`` too with a window), ``num_items``,
   ``max_q_len`` - no item has more new tokens -, ``max_ctx_len`` and ``scratch``: a ``Workspace``, which one call uses at a time.  Without it a
