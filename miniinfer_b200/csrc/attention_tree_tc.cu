@@ -21,7 +21,7 @@
 //
 // Measured, heads of 128: 32 trees of 64 over up to 8192 keys, 32 heads on 8 (625 MB, 105 GFLOP) 180 us in short bursts, 200 to 215 one call after the other (the power cap): 3.5 and 2.9 to 3.1 TB/s; 8 trees of 32 over up to
 // 4096 keys (62 MB) 24 to 26 us, with a cap of 30 37.5, with pages of 16 30.5, heads of 64 and 256 21.8 and 40.3; one tree of 8 over 2047 keys, 16 heads on 8 (8.5 MB) 16.5 us.  The first is
-// bound by the chain from scores over exponentials to weights (with a cap, two more operations of the exponentials' unit a score, 404 us): two sets of rows leave the tensor cores 35 % busy,
+// bound by the chain from scores over exponentials to weights (with a cap, whose exponentials and reciprocals come on top, 404 us): two sets of rows leave the tensor cores 35 % busy,
 // without the softmax the products and copies alone took 130 us.  The others are bound by what a
 // piece costs whatever its length is - its description, its queries, the first tile's latency, its sums - about 4000 cycles, and 10000 once a block.
 #include <cuda.h>

@@ -14,7 +14,7 @@
 //
 // Measured: 96 pages of 28 layers (1.41 GB read and written) 216 us, 6.5 TB/s, the rate of a plain copy; paths of 8 of 64 tokens for 64 requests (117 MB)
 // 20.5 us, 5.7 TB/s; 32 states of 12 layers of 1 MB 81 us (what keeps its place costs nothing); 3 pages (15 MB) 6.9 us; calls of a MB or less 1.7 to 2.5 us,
-// which a launch takes.  Rows that are not whole 16 bytes are copied by 4 or 2 bytes: 32 states of 12 layers of 95151 float32 77 us, 49 % of the bytes' rate.
+// which a launch takes.  Rows that are not whole 16 bytes are copied by 4 or 2 bytes: 32 states of 12 layers of 95151 float32 77 us, 38 % of the bytes' rate.
 #include "common.cuh"
 
 namespace {
